@@ -85,7 +85,7 @@ class _Hip:
                      "spy_norm_pair_mean", "spy_scale_cap", "spy_result_norm", "spy_moe_align_tables", "spy_layer_norm", "spy_layer_norm_residual",
                      "spy_gelu", "spy_norm_rope_store", "spy_map_difference", "spy_rotation_angles", "spy_decay_memory", "spy_group_norm", "spy_gemm_rows",
                      "spy_add_parts_rmsnorm", "spy_gemm_f32_parts", "spy_gemm_f32_gated", "spy_gemm_f32_into", "spy_gemm_f32_into_parts",
-                     "spy_gemm_f32_scaled"):
+                     "spy_gemm_f32_scaled", "spy_add_rmsnorm_q8", "spy_quantize_rows", "spy_gemm_q8"):
             if not hasattr(self.lib, name):
                 raise KernelError("the kernel library %s lacks %s: it is older than its sources; build it again "
                                   "(spyinfer_amd.kernels.build.build())" % (self.lib._name, name))
@@ -94,6 +94,9 @@ class _Hip:
         # ctypes object per argument: 3 us of the host's 14 per call)
         P, I = ctypes.c_void_p, ctypes.c_int
         self.lib.spy_gemm_decode.argtypes = [P, I, P, I, ctypes.c_float, P, I, P, I, P, P, P, P, I, I, I, I, I, I, P, ctypes.c_int64, I, P]
+        self.lib.spy_gemm_q8.argtypes = [P, I, P, ctypes.c_int64, P, P, P, I, I, I, I, I, I, P]
+        self.lib.spy_add_rmsnorm_q8.argtypes = [P, P, P, P, I, P, I, ctypes.c_float, I, I, ctypes.c_int64, P]
+        self.lib.spy_quantize_rows.argtypes = [P, P, P, I, ctypes.c_int64, I, I, ctypes.c_int64, P]
 
     def call(self, name, *args):
         rc = getattr(self.lib, name)(*args)
@@ -115,6 +118,14 @@ class _Hip:
         # torch's current HIP stream of the current device, by the two calls that do no more than read it (the Stream
         # object of torch.cuda.current_stream() costs 3 us to build, and a step has hundreds of launches)
         return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on_device_of(t: torch.Tensor):
+    """Launches inside go to the current stream of the device that ``t`` lies on."""
+    return _HERE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def hip() -> _Hip:
@@ -2691,6 +2702,165 @@ def moe_experts(x: torch.Tensor, ids: Optional[torch.Tensor], weights: Optional[
                ctypes.c_int(per_block), ctypes.c_int(0), ctypes.c_float(0.0), _ptr(None), _Hip.stream())
     result = ExpertRows(y, pair_row, None if weight_input else weights, add, top, scale, T, x.dtype)
     return result if unsummed else result.combine()
+
+
+# --------------------------------------------------------------------------
+# Products in 8-bit integers
+
+#: widest rows of a product in 8-bit integers: its sums stay within 32 bits
+Q8_MAX_WIDTH = 511 * 256
+
+
+def _q8_pitch(width: int) -> int:
+    return (width + 15) & ~15
+
+
+class Q8Rows:
+    """Rows in 8-bit integers: row t stands for ``values[t, :width]`` times ``scales[t]``.  ``values`` int8 [T, pitch], pitch the
+    width rounded up to 16 (what lies behind a row's end is anything); ``scales`` float32 [T]."""
+    __slots__ = ("values", "scales", "width")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, width: int):
+        self.values, self.scales, self.width = values, scales, width
+
+    shape = property(lambda self: (self.values.shape[0], self.width))
+    device = property(lambda self: self.values.device)
+
+    @staticmethod
+    def from_values(values: torch.Tensor, scales: torch.Tensor) -> "Q8Rows":
+        """``values`` int8 [T, K] with a scale for each row, float32 [T]."""
+        _check(values.dim() == 2 and values.dtype == torch.int8 and values.shape[1] > 0, "Q8Rows: int8 values [T, K] expected")
+        _check(tuple(scales.shape) == (values.shape[0],) and scales.dtype == torch.float32, "Q8Rows: a float32 scale for each row expected")
+        T, K = values.shape
+        if K % 16 or not values.is_contiguous() or values.data_ptr() % 16:
+            kept = torch.zeros((T, _q8_pitch(K)), dtype=torch.int8, device=values.device)
+            kept[:, :K] = values
+            values = kept
+        _dev(values, scales)
+        return Q8Rows(values, scales, K)
+
+    def to_rows(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values that the rows stand for, [T, K], each rounded once to ``dtype``."""
+        return (self.values[:, :self.width].double() * self.scales[:, None]).to(dtype)
+
+
+class Q8Weight:
+    """A matrix [N, K] of 8-bit integers with a float32 scale for each row, laid out for the products: row n stands for its
+    integers times ``scales[n]``.  ``gated``: the rows are [gate | up], N / 2 each.  ``tiles``: the integers in the order in which the
+    matrix instructions take them (csrc/q8.h), K filled up to 256 and the rows (of each half) to 16 with zeros; ``scales`` has
+    an entry for each row of ``tiles``, zeros for those filled up."""
+    __slots__ = ("tiles", "scales", "shape", "gated")
+
+    device = property(lambda self: self.tiles.device)
+    is_cuda = property(lambda self: self.tiles.is_cuda)
+    dtype = torch.int8
+
+    def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, shape, gated: bool):
+        self.tiles, self.scales, self.shape, self.gated = tiles, scales, torch.Size(shape), gated
+
+    def dim(self) -> int:
+        return 2
+
+    @staticmethod
+    def from_values(values: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> "Q8Weight":
+        """``values`` int8 [N, K] with a finite scale for each row, float32 [N]."""
+        _check(values.dim() == 2 and values.dtype == torch.int8 and values.numel() > 0, "Q8Weight: int8 values [N, K] expected")
+        _check(tuple(scales.shape) == (values.shape[0],) and scales.dtype == torch.float32 and scales.device == values.device,
+               "Q8Weight: a float32 scale for each row expected")
+        N, K = values.shape
+        halves = 2 if gated else 1
+        _check(N % halves == 0, "Q8Weight: %d rows are no gate and up rows", N)
+        _check(K <= Q8_MAX_WIDTH, "Q8Weight: a width of %d, the sums hold %d", K, Q8_MAX_WIDTH)
+        _check(bool(torch.isfinite(scales).all()), "Q8Weight: a row's scale is no finite number")
+        rows, width = -(-(N // halves) // 16) * 16, -(-K // 256) * 256
+        _check(halves * rows * width < 1 << 31, "Q8Weight: a matrix of %d x %d is too large", N, K)
+        full = values.new_zeros((halves, rows, width))
+        full[:, :N // halves, :K] = values.view(halves, N // halves, K)
+        tiles = full.view(halves * rows // 16, 16, width // 256, 4, 4, 16).permute(2, 0, 3, 4, 1, 5).contiguous()
+        kept = scales.new_zeros((halves, rows))
+        kept[:, :N // halves] = scales.view(halves, N // halves)
+        return Q8Weight(tiles, kept.view(-1), (N, K), bool(gated))
+
+    def to_rows(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The matrix that the integers stand for, [N, K], each value rounded once to ``dtype``."""
+        N, K = self.shape
+        halves = 2 if self.gated else 1
+        chunks, tiles = self.tiles.shape[:2]
+        full = self.tiles.permute(1, 4, 0, 2, 3, 5).reshape(halves, tiles * 16 // halves, chunks * 256).double() * self.scales.view(halves, -1, 1)
+        return full[:, :N // halves, :K].reshape(N, K).to(dtype)
+
+
+def quantize_weight(w: torch.Tensor, gated: bool = False) -> Q8Weight:
+    """``w [N, K]`` (float32 or bfloat16) as a ``Q8Weight``: every row's integers are 127 w / max |w| rounded half to even, its
+    scale max |w| / 127."""
+    rows = quantize_rows(w)
+    return Q8Weight.from_values(rows.values[:, :rows.width].contiguous(), rows.scales, gated)
+
+
+def quantize_rows(x: torch.Tensor) -> Q8Rows:
+    """Rows ``x [T, K]`` (float32 or bfloat16; they may be a view into the rows of a wider tensor) in 8-bit integers: 127 x / a rounded half to
+    even, a = max |x| of the row, and the scale a / 127.  A row of zeros has zeros and the scale 0; one with a NaN or an infinity zeros and the
+    scale NaN, so that all that is made of it is NaN."""
+    _check(x.is_cuda and x.dim() == 2 and x.dtype in _CODES and x.shape[1] > 0, "quantize_rows: float32 or bfloat16 rows [T, K] on the GPU expected")
+    T, K = x.shape
+    _check(T <= 1 or (x.stride(1) == 1 or K == 1) and x.stride(0) >= K, "quantize_rows: dense rows, or rows of a wider tensor, expected")
+    _check(T > 1 or K == 1 or x.stride(1) == 1, "quantize_rows: dense rows, or rows of a wider tensor, expected")
+    with _on_device_of(x):
+        values = torch.empty((T, _q8_pitch(K)), dtype=torch.int8, device=x.device)
+        scales = torch.empty((T,), dtype=torch.float32, device=x.device)
+        if T:
+            hip().call("spy_quantize_rows", values.data_ptr(), scales.data_ptr(), x.data_ptr(), _CODES[x.dtype], max(x.stride(0), K) if T > 1 else K, T, K,
+                       values.shape[1], _Hip.stream())
+    return Q8Rows(values, scales, K)
+
+
+def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, eps: float) -> Q8Rows:
+    """resid += delta (float32, in place; skipped if delta is None), then the RMS norm of the sum in 8-bit integers with a scale for
+    each row, as ``quantize_rows`` has them (of the norm's result in full, not of one rounded to bfloat16).  ``delta``: [T, H] float32 or
+    bfloat16."""
+    _dev(resid, delta, weight)
+    _check(resid.dtype == torch.float32 and resid.dim() == 2 and resid.shape[1] > 0, "add_rms_norm_q8: the residual stream must be float32 [T, H]")
+    T, H = resid.shape
+    _check(weight.shape == (H,) and weight.dtype in _CODES, "add_rms_norm_q8: weight must be [H], float32 or bfloat16")
+    _check(delta is None or (delta.shape == resid.shape and delta.dtype in _CODES), "add_rms_norm_q8: delta must be [T, H], float32 or bfloat16")
+    with _on_device_of(resid):
+        values = torch.empty((T, _q8_pitch(H)), dtype=torch.int8, device=resid.device)
+        scales = torch.empty((T,), dtype=torch.float32, device=resid.device)
+        if T:
+            hip().call("spy_add_rmsnorm_q8", values.data_ptr(), scales.data_ptr(), resid.data_ptr(), 0 if delta is None else delta.data_ptr(),
+                       0 if delta is None else _CODES[delta.dtype], weight.data_ptr(), _CODES[weight.dtype], eps, T, H, values.shape[1], _Hip.stream())
+    return Q8Rows(values, scales, H)
+
+
+def _gemm_q8(x: Q8Rows, w: Q8Weight, out: torch.Tensor, columns: int, act: int) -> torch.Tensor:
+    if out.shape[0]:
+        with _on_device_of(out):
+            hip().call("spy_gemm_q8", out.data_ptr(), _CODES[out.dtype], x.values.data_ptr(), x.values.shape[1], x.scales.data_ptr(), w.tiles.data_ptr(),
+                       w.scales.data_ptr(), out.shape[0], columns, w.tiles.shape[1], w.tiles.shape[0], 1 if w.gated else 0, act, _Hip.stream())
+    return out
+
+
+def linear_q8(x: Q8Rows, w: Q8Weight, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y = x . w^T of rows and a matrix in 8-bit integers: the sums of products are 32-bit integers, exact; a sum times its row's and
+    its column's scale is rounded once, to ``out_dtype`` (bfloat16 or float32).  ``out``: the result is written there."""
+    _check(isinstance(x, Q8Rows) and isinstance(w, Q8Weight), "linear_q8: Q8Rows and a Q8Weight expected")
+    _check(not w.gated, "linear_q8: a matrix of gate and up rows goes to linear_q8_gated")
+    _check(x.width == w.shape[1], "linear_q8: rows of %d and a matrix of %d x %d", x.width, w.shape[0], w.shape[1])
+    _check(out_dtype in _CODES, "linear_q8: output dtype must be float32 or bfloat16")
+    _dev(x.values, x.scales, w.tiles, w.scales)
+    return _gemm_q8(x, w, _result(out, x.values.shape[0], w.shape[0], out_dtype, x.values.device), w.shape[0], 0)
+
+
+def linear_q8_gated(x: Q8Rows, w: Q8Weight, activation: str = "silu") -> torch.Tensor:
+    """act(x . Wgate^T) * (x . Wup^T) -> bfloat16 [M, N / 2] for a matrix of [gate | up] rows, the two values formed as in
+    ``linear_q8`` and rounded once, after the activation.  ``activation``: one of GATED_ACTIVATIONS."""
+    _check(isinstance(x, Q8Rows) and isinstance(w, Q8Weight), "linear_q8_gated: Q8Rows and a Q8Weight expected")
+    _check(w.gated, "linear_q8_gated: a matrix of [gate | up] rows expected")
+    _check(x.width == w.shape[1], "linear_q8_gated: rows of %d and a matrix of %d x %d", x.width, w.shape[0], w.shape[1])
+    _check(activation in GATED_ACTIVATIONS, "linear_q8_gated: activation %r is not implemented", activation)
+    _dev(x.values, x.scales, w.tiles, w.scales)
+    out = torch.empty((x.values.shape[0], w.shape[0] // 2), dtype=torch.bfloat16, device=x.values.device)
+    return _gemm_q8(x, w, out, w.shape[0] // 2, GATED_ACTIVATIONS[activation])
 
 
 # --------------------------------------------------------------------------
