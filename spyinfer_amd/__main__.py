@@ -34,6 +34,8 @@ def main(argv=None) -> int:
     ap.add_argument("--num-kvcache-blocks", type=int, default=None)
     ap.add_argument("--weight-copies", default="both", choices=["both", "tiled"],
                     help="tiled: matrices are kept in tiles only (half the weights' memory, prompts a sixth slower)")
+    ap.add_argument("--matrix-precision", default="stored", choices=["stored", "int8"],
+                    help="int8: the matrices of the attention and of the gated feed-forwards as 8-bit integers (bfloat16 only)")
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--max-new-tokens", type=int, default=None)
@@ -69,7 +71,7 @@ def main(argv=None) -> int:
                        keep_finished_cache=False,
                        gpu_memory_utilization=args.gpu_memory_utilization, enforce_eager=args.enforce_eager,
                        kvcache_block_size=args.kvcache_block_size, num_kvcache_blocks=args.num_kvcache_blocks, seed=args.seed,
-                       weight_copies=args.weight_copies)
+                       weight_copies=args.weight_copies, matrix_precision=args.matrix_precision)
     params = SamplingParams(temperature=args.temperature, max_new_tokens=args.max_new_tokens, ignore_eos=args.ignore_eos)
 
     def stream(rid):

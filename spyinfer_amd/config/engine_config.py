@@ -43,6 +43,12 @@ class EngineConfig:
     #: then restores each matrix's rows into a scratch tensor ahead of its product (a prompt portion of 2048 tokens
     #: takes about a sixth longer).  Matrices without a tiled form (float32, odd shapes) keep their rows either way.
     weight_copies: str = "both"
+    #: "stored": matrices have the precision of the model folder.  "int8": those of the attention and of the gated
+    #: feed-forwards are held as 8-bit integers with a scale for each output channel, and their products are integer
+    #: products with rows brought to 8 bits as they come, a scale for each token; half the memory and the bytes of a
+    #: decode step, at the precision of 8-bit weights and activations.  bfloat16 engines only; the embedding, the output
+    #: head and all other matrices stay as they are.
+    matrix_precision: str = "stored"
 
     def validate(self) -> None:
         if self.dtype not in ("bfloat16", "float32"):
@@ -54,5 +60,9 @@ class EngineConfig:
             raise ValueError("num_kvcache_blocks must be positive")
         if self.weight_copies not in ("both", "tiled"):
             raise ValueError("weight_copies must be 'both' or 'tiled', got %r" % (self.weight_copies,))
+        if self.matrix_precision not in ("stored", "int8"):
+            raise ValueError("matrix_precision must be 'stored' or 'int8', got %r" % (self.matrix_precision,))
+        if self.matrix_precision == "int8" and self.dtype != "bfloat16":
+            raise ValueError("matrix_precision 'int8' goes with dtype 'bfloat16': a float32 engine computes in 32 bits throughout")
         if not (0.0 < self.gpu_memory_utilization <= 1.0):
             raise ValueError("gpu_memory_utilization must be in (0, 1]")

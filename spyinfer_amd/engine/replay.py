@@ -40,6 +40,8 @@ def run(argv=None, stdin=None, stdout=None) -> int:
                     help="most tokens that live requests hold at any time (each rounded up to a multiple of 64)")
     ap.add_argument("--kvcache-block-size", type=int, default=16, help="tokens in a cache page")
     ap.add_argument("--max-num-seqs", type=int, default=4, help="most live requests (state slots)")
+    ap.add_argument("--matrix-precision", default="stored", choices=["stored", "int8"],
+                    help="int8: the matrices of the attention and of the gated feed-forwards as 8-bit integers (bfloat16 only)")
     ap.add_argument("--device", default="cuda:0")
     ap.add_argument("--poison-cache", action="store_true",
                     help="fill the cache pool with NaN before the first step: a read of a slot that no step wrote shows in the logits")
@@ -55,7 +57,7 @@ def run(argv=None, stdin=None, stdout=None) -> int:
     if args.max_tokens <= 0:
         ap.error("--max-tokens must be positive")
     ops.hip()       # builds the kernel library at the first call, and fails here if there is no GPU
-    model = load_model(args.model, args.dtype, args.device)
+    model = load_model(args.model, args.dtype, args.device, matrix_precision=args.matrix_precision)
     num_pages = page_rounded_tokens(args.max_tokens, args.kvcache_block_size)
     runner = ModelRunner(model, args.dtype, args.device, args.kvcache_block_size, num_pages, args.max_num_seqs,
                          max_num_batched_tokens=1 << 30)

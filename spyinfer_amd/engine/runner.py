@@ -34,22 +34,28 @@ def resolve_dtype(name) -> torch.dtype:
     return DTYPES[name]
 
 
-def bind_weights(model: DecoderModel, weights, device, weight_copies: str = "both") -> None:
-    """``model.bind`` with the engine's choice of the forms in which matrices are kept (EngineConfig.weight_copies)."""
-    before = ops.ROW_MAJOR_WEIGHTS
-    ops.ROW_MAJOR_WEIGHTS = weight_copies != "tiled"
+def bind_weights(model: DecoderModel, weights, device, weight_copies: str = "both", matrix_precision: str = "stored") -> None:
+    """``model.bind`` with the engine's choice of the forms in which matrices are kept (EngineConfig.weight_copies,
+    EngineConfig.matrix_precision)."""
+    before = ops.ROW_MAJOR_WEIGHTS, ops.MATRICES_Q8
+    ops.ROW_MAJOR_WEIGHTS, ops.MATRICES_Q8 = weight_copies != "tiled", matrix_precision == "int8"
+    kept = ops.matrices_kept_q8()
     try:
         model.bind(weights, device)
     finally:
-        ops.ROW_MAJOR_WEIGHTS = before
+        ops.ROW_MAJOR_WEIGHTS, ops.MATRICES_Q8 = before
+    if matrix_precision == "int8" and ops.matrices_kept_q8() == kept:
+        raise ValueError("matrix_precision 'int8': the model has no matrix that can be held in 8 bits (those of PagedAttention and GatedMLP can)")
 
 
-def load_model(folder: str, dtype, device, weight_copies: str = "both") -> DecoderModel:
+def load_model(folder: str, dtype, device, weight_copies: str = "both", matrix_precision: str = "stored") -> DecoderModel:
     """config.json -> architecture -> model of parts, weights bound by name."""
     arch, cfg = load_model_config(folder)
     model = arch.build(cfg)
+    if matrix_precision == "int8" and resolve_dtype(dtype) != torch.bfloat16:
+        raise ValueError("matrix_precision 'int8' goes with dtype 'bfloat16': a float32 model computes in 32 bits throughout")
     weights = load_weights(folder, model.weight_specs(), resolve_dtype(dtype), device)
-    bind_weights(model, weights, device, weight_copies)
+    bind_weights(model, weights, device, weight_copies, matrix_precision)
     return model
 
 

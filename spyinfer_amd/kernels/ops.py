@@ -417,10 +417,27 @@ class TiledOnly:
         return untile_weight(t, self._buf[:t.numel()].view(t.shape))
 
 
-def weight_forms(w: torch.Tensor, keep_rows: bool = False):
+#: True while a model's weights are bound: the matrices of the parts that ask for it are kept in 8-bit integers only
+MATRICES_Q8 = False
+_q8_kept = 0                  # matrices kept so since the process began
+
+
+def matrices_kept_q8() -> int:
+    """How many matrices ``weight_forms`` has brought to 8 bits in this process: what binding a model adds to it is the
+    model's share."""
+    return _q8_kept
+
+
+def weight_forms(w: torch.Tensor, keep_rows: bool = False, q8: bool = False, gated: bool = False):
     """(matrix, tiled copy or None) as a part keeps them for ``linear``: both forms, or, with ROW_MAJOR_WEIGHTS off and
     a tiled copy at hand, the tiled copy alone (the first member is then a TiledOnly).  ``keep_rows``: the rows are
-    needed for something else than products (an embedding table) and stay."""
+    needed for something else than products (an embedding table) and stay.  ``q8``: with MATRICES_Q8 on the matrix is
+    kept as a ``Q8Weight`` alone (``gated``: of [gate | up] rows), which ``linear``, ``linear_few``, ``linear_parts`` and
+    ``linear_swiglu`` take in a matrix' place."""
+    global _q8_kept
+    if q8 and MATRICES_Q8:
+        _q8_kept += 1
+        return quantize_weight(w, gated), None
     tiled = tile_weight(w)
     if tiled is not None and not ROW_MAJOR_WEIGHTS and not keep_rows:
         return TiledOnly(tiled), tiled
@@ -444,7 +461,10 @@ def linear(x: torch.Tensor, w: torch.Tensor, out_dtype: Optional[torch.dtype] = 
 
     float32 anywhere among x and w -> the hand-written true-fp32 kernels.  All of it float32: the kernel, and with it the
     order of a row's sums, goes by the number of rows (csrc/gemm_f32.hip), so that a row of another batch is the same within
-    rounding and not bit for bit.  All bfloat16: the streaming MFMA kernel for few rows, the library product for many."""
+    rounding and not bit for bit.  All bfloat16: the streaming MFMA kernel for few rows, the library product for many.
+    ``w`` a ``Q8Weight``: ``linear_q8`` of ``x``, which is brought to 8 bits first unless it is ``Q8Rows``."""
+    if isinstance(w, Q8Weight):
+        return linear_q8(_q8_rows(x), w, out_dtype or (torch.bfloat16 if isinstance(x, Q8Rows) else x.dtype), out)
     _dev(x, w)
     _check(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], "linear: x [M, K] and w [N, K] expected, got %s and %s"
            % (tuple(x.shape), tuple(w.shape)))
@@ -504,6 +524,8 @@ def linear_few(x: torch.Tensor, w: torch.Tensor, tiled: Optional[torch.Tensor] =
     """``linear`` for parts that do not fold norms into their products: up to DECODE_ROWS_PLAIN bfloat16 rows go to the
     decode products (which stream the tiled matrix once and beat the library there: 18.7 against 20.3 us for 6144 x 4096 at
     32 rows, 10.5 against 20.6 for 4096 x 4096), everything else to ``linear``."""
+    if isinstance(w, Q8Weight):
+        return linear(x, w, out_dtype, out=out)
     if tiled is not None and x.dtype == torch.bfloat16 and x.dim() == 2 and 0 < x.shape[0] <= DECODE_ROWS_PLAIN and x.is_contiguous() \
             and not (out_dtype == torch.float32 and rows_product_logits(x.shape[0], w.shape[0], w.shape[1])):
         return decode_linear(x, tiled, out_dtype or torch.bfloat16, out)
@@ -794,6 +816,8 @@ class ProductParts:
 
 def linear_parts(x: torch.Tensor, w: torch.Tensor, tiled: Optional[torch.Tensor] = None):
     """``linear_few``, or, where a product of many rows is better cut along K, its ``ProductParts``."""
+    if isinstance(w, Q8Weight):
+        return linear(x, w)
     M, K = x.shape
     if M <= (8 if x.dtype == torch.float32 else 16):      # (short steps are bound by their launches: nothing more is asked of them)
         return linear_few(x, w, tiled)
@@ -846,7 +870,10 @@ def linear_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, tiled: Optional[torc
                   activation: str = "silu") -> torch.Tensor:
     """act(x . Wgate^T) * (x . Wup^T) with ``w_gate_up [2 I, K]`` = [Wgate | Wup] -> [M, I].  For few bfloat16 rows
     (decode), and for most sizes of many, one kernel does both products and the activation; otherwise it is linear() followed by swiglu().  ``few_rows``:
-    most rows that the tiled kernel takes here (0: SKINNY_MAX_ROWS).  ``activation``: one of GATED_ACTIVATIONS."""
+    most rows that the tiled kernel takes here (0: SKINNY_MAX_ROWS).  ``activation``: one of GATED_ACTIVATIONS.  ``w_gate_up`` a
+    ``Q8Weight``: ``linear_q8_gated``."""
+    if isinstance(w_gate_up, Q8Weight):
+        return linear_q8_gated(_q8_rows(x), w_gate_up, activation)
     _dev(x, w_gate_up)
     _check(x.dim() == 2 and w_gate_up.dim() == 2 and x.shape[1] == w_gate_up.shape[1] and w_gate_up.shape[0] % 2 == 0,
            "linear_swiglu: x [M, K] and w [2 I, K] expected")
@@ -2812,6 +2839,10 @@ def quantize_rows(x: torch.Tensor) -> Q8Rows:
             hip().call("spy_quantize_rows", values.data_ptr(), scales.data_ptr(), x.data_ptr(), _CODES[x.dtype], max(x.stride(0), K) if T > 1 else K, T, K,
                        values.shape[1], _Hip.stream())
     return Q8Rows(values, scales, K)
+
+
+def _q8_rows(x) -> Q8Rows:
+    return x if isinstance(x, Q8Rows) else quantize_rows(x)
 
 
 def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor, eps: float) -> Q8Rows:

@@ -234,11 +234,11 @@ class PagedAttention(Mixer):
         # one product for q, k and v (and the gate): rows [q heads | k heads | v heads | gate]
         self.w_qkv = torch.cat(mats, dim=0).contiguous()
         del mats
-        self.w_qkv, self.w_qkv_tiled = ops.weight_forms(self.w_qkv)
+        self.w_qkv, self.w_qkv_tiled = ops.weight_forms(self.w_qkv, q8=True)
         w_o = weights.pop(prefix + n["o"])
         if dv != self.head_dim:
             w_o = self._padded(w_o.t().contiguous(), nq, dv).t().contiguous()
-        self.w_o, self.w_o_tiled = ops.weight_forms(w_o)
+        self.w_o, self.w_o_tiled = ops.weight_forms(w_o, q8=True)
         if self.has_bias:
             b = [weights[prefix + n[c] + n["bias"]] for c in "qkv"]
             if len({t.dtype for t in b}) > 1:
@@ -262,6 +262,10 @@ class PagedAttention(Mixer):
                 self.q_norm, self.k_norm = self.q_norm.float(), self.k_norm.float()
         if self.position is not None and not self._plain_projections():
             self.position.prepare(self.w_o.device, 0)
+
+    @property
+    def takes_q8_rows(self):
+        return isinstance(self.w_qkv, ops.Q8Weight) and type(self).forward is PagedAttention.forward
 
     # ---- cache -----------------------------------------------------------
     def cache_spec(self):

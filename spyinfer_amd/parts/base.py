@@ -51,6 +51,11 @@ class Norm(Part):
         the hidden state."""
         raise NotImplementedError
 
+    def gives_q8_rows(self, delta) -> bool:
+        """Whether ``add_norm_q8(resid, delta)`` exists and takes ``delta``: ``add_norm`` of all rows, its result in 8-bit
+        integers with a scale for each row (``ops.Q8Rows``)."""
+        return False
+
     def add_normed(self, base: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None, copy_dtype=None, mix=None):
         """out = base + norm(y), float32, for blocks that norm a sublayer's output; (out, copy in ``copy_dtype`` or None).
         ``mix`` = (kept layer results, n, weights): also the weighted sum of the n kept results, of which ``out`` is the
@@ -83,6 +88,9 @@ class PositionEncoding(Part):
 class Mixer(Part):
     """Mixes information between the tokens of a request (attention here)."""
 
+    #: ``forward`` takes rows in 8-bit integers (``ops.Q8Rows``) in place of x
+    takes_q8_rows = False
+
     def cache_spec(self):
         """``PagedKV``, ``FixedState`` or None: what one layer of this mixer keeps per request."""
         return None
@@ -113,6 +121,9 @@ class Mixer(Part):
 
 
 class FeedForward(Part):
+    #: as ``Mixer.takes_q8_rows``
+    takes_q8_rows = False
+
     def forward(self, x: torch.Tensor, batch) -> torch.Tensor:
         """x [T, H] (normed) -> [T, H]."""
         raise NotImplementedError

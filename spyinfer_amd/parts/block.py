@@ -95,6 +95,13 @@ class PreNormBlock(Block):
     def capturable(self, batch):
         return all(part.capturable(batch) for part, _ in self._parts(""))
 
+    @staticmethod
+    def _normed(norm, part, resid, delta, act):
+        """``norm.add_norm``, in 8-bit integers where the part that reads the result (None: others read it too) takes them."""
+        if part is not None and part.takes_q8_rows and norm.gives_q8_rows(delta):
+            return norm.add_norm_q8(resid, delta)
+        return norm.add_norm(resid, delta, act)
+
     def forward(self, resid, pending, batch, cache, store=True, next_norm=None):
         act = batch.act_dtype
         ready = isinstance(pending, ops.ScaledInput)
@@ -116,7 +123,7 @@ class PreNormBlock(Block):
             if next_norm is not None and next_norm.foldable(act) is not None:
                 return resid, self.ffn.forward_into(n2, batch, resid, next_norm)
             return resid, self.ffn.forward(n2, batch)
-        n1 = self.norm1.add_norm(resid, None if ready else pending, act)
+        n1 = self._normed(self.norm1, self.mixer if self.gate1 is None else None, resid, None if ready else pending, act)
         # (a result in parts goes to the norm that sums them: to the next block's only if that one is known)
         in_parts = self.gate1 is None and hasattr(self.mixer, "forward_parts") \
             and getattr(next_norm if self.ffn is None else self.norm2, "takes_product_parts", False)
@@ -125,7 +132,7 @@ class PreNormBlock(Block):
             a = self.gate1.apply(a, n1)
         if self.ffn is None:
             return resid, a
-        n2 = self.norm2.add_norm(resid, a, act)
+        n2 = self._normed(self.norm2, self.ffn if self.gate2 is None else None, resid, a, act)
         if self.gate2 is None and hasattr(self.ffn, "forward_parts") and getattr(next_norm, "takes_product_parts", False):
             return resid, self.ffn.forward_parts(n2, batch)
         if getattr(self.gate2, "takes_expert_rows", False) and hasattr(self.ffn, "forward_unsummed"):

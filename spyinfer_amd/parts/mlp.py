@@ -43,9 +43,13 @@ class GatedMLP(FeedForward):
         self.w_gate_up = torch.cat([g, u], dim=0).contiguous()
         del g, u
         # tiles 0 .. I/16 - 1 of the tiled copy are gate rows, the rest up rows: what the fused SwiGLU kernel expects
-        if self.intermediate_size % 16 == 0:
-            self.w_gate_up, self.w_gate_up_tiled = ops.weight_forms(self.w_gate_up)
-        self.w_down, self.w_down_tiled = ops.weight_forms(weights.pop(down))
+        if self.intermediate_size % 16 == 0 or ops.MATRICES_Q8:
+            self.w_gate_up, self.w_gate_up_tiled = ops.weight_forms(self.w_gate_up, q8=True, gated=True)
+        self.w_down, self.w_down_tiled = ops.weight_forms(weights.pop(down), q8=True)
+
+    @property
+    def takes_q8_rows(self):
+        return isinstance(self.w_gate_up, ops.Q8Weight) and type(self).forward is GatedMLP.forward
 
     def capturable(self, batch):
         return True

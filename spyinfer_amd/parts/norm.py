@@ -92,6 +92,12 @@ class RMSNorm(Norm):
             return ops.add_rms_norm(resid, first, self.weight, self.eps, out_dtype, rows, delta2=second, groups=self.groups)
         return ops.add_rms_norm(resid, delta, self.weight, self.eps, out_dtype, rows, groups=self.groups)
 
+    def gives_q8_rows(self, delta):
+        return type(self).add_norm is RMSNorm.add_norm and self.groups == 1 and (delta is None or isinstance(delta, torch.Tensor))
+
+    def add_norm_q8(self, resid, delta):
+        return ops.add_rms_norm_q8(resid, delta, self.weight, self.eps)
+
     def add_normed(self, base, y, out=None, copy_dtype=None, mix=None):
         """out = base + norm(y) in float32 (the norm on a sublayer's output; ``out`` may be ``base``); returns (out, its
         copy in ``copy_dtype`` or None).  ``mix`` = (kept results [layers, T, H], n, weights [n]) with ``out`` the n-th
