@@ -1,6 +1,6 @@
 // Products of 8-bit integer rows with 8-bit integer matrices (q8.h has both forms), sums in 32-bit integers, which hold them exactly
 // (K < 2^17):  y[m][n] = sum * row scale * column scale, rounded once; or the gated pair of such values.
-#include "q8.h"
+#include "gemm_q8.h"
 
 #define Q8_WAVES 4
 
@@ -78,6 +78,7 @@ extern "C" int spy_gemm_q8(void* C, int c_dtype, const void* X, int64_t pitch, c
     SPY_REQUIRE((((uintptr_t)X | (uintptr_t)W) % 16) == 0, "spy_gemm_q8: operands must be 16-byte aligned");
     SPY_REQUIRE(!gated || (gate_act_of(act_code, &act) && c_dtype == SPY_BF16), "spy_gemm_q8: activation %d, result dtype %d", act_code, c_dtype);
     SPY_REQUIRE(M <= 65535 * 64, "spy_gemm_q8: too many rows");
+    if (M > 512) return q8_tall_launch(C, c_dtype, (const int8_t*)X, pitch, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, 16, st);
 #define Q8(MT, EPI, TC) gemm_q8_kernel<MT, EPI, TC><<<dim3(EPI == Q8_GATED ? tiles / 2 : tiles, (M + 16 * MT - 1) / (16 * MT)), Q8_WAVES * 64, 0, st>>>( \
         (TC*)C, (const int8_t*)X, pitch, sx, (const int8_t*)W, sw, M, N, tiles, chunks, act)
     if (gated) { if (M <= 16) Q8(1, Q8_GATED, bf16_t); else Q8(4, Q8_GATED, bf16_t); }

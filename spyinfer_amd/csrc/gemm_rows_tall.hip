@@ -20,6 +20,7 @@
 // What bounds it: at thirteen row tiles the matrix units are busy for 88 % of a turn and the clock falls to 1.6 to 1.9 GHz; at nine a turn's loads,
 // 26 % over its products, and a block's way in (2.2 us to its first turn) and out (2 to 4 us), which a lone wave a SIMD shows.
 #include "gemm_rows.h"
+#include "gemm_tall.h"
 
 // Two products of a row tile, X's 16 rows with two column tiles of W.  The compiler does not see matrix instructions here and leaves out the
 // wait states between them and ordinary instructions: an operand's register that one has written needs two (a turn begins with them, and
@@ -28,84 +29,11 @@
 __device__ __forceinline__ void gr_mfma2(gr_f32x4_t& a, gr_f32x4_t& b, gr_bf16x8_t w0, gr_bf16x8_t w1, gr_bf16x8_t x) {
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %2, %4, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %3, %4, %1" : "+a"(a), "+a"(b) : "v"(w0), "v"(w1), "v"(x));
 }
-__device__ __forceinline__ void gr_sums_settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
-
-// All turns of a block: n of them, of 128 of K.  wres, w_lane, w_at, w_turn: W's buffer, this lane's bytes in a load, each column tile's place and a
-// turn's bytes.  load_x(stage, i, c): asks for row tile i of turn c, straight into LDS (a wave 4 of its 16 rows).  Ends with nothing under way,
-// the stages free and the sums fit to be read.  MT: 8 to 16.
-template <int MT, typename RES, typename X>
-__device__ __forceinline__ void gr_tall_turns(gr_f32x4_t (&acc)[4][MT], RES wres, int w_lane, const int (&w_at)[4], int w_turn, int n, bf16_t* stage0, bf16_t* stage1,
-                                              int lane, X load_x) {
-    // (two arrays of their own: reads of a stage that the compiler cannot tell from the one that loads go to wait for these)
-    static_assert(MT >= 8 && MT <= 16, "eight loads of W go between the row tiles of a step");
-    const int r = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[j][i] = gr_f32x4_t{0.f, 0.f, 0.f, 0.f};
-    gr_bf16x8_t w[2][4][4];
-    auto load_w = [&](int d, int s, int j, int c) {
-        w[d][s][j] = __builtin_bit_cast(gr_bf16x8_t, __builtin_amdgcn_raw_buffer_load_b128(wres, w_lane, w_at[j] + c * w_turn + s * 1024, 0));
-    };
-    // The products of a turn with w[d].  Between them, one load a row tile: X of turn `next` into the other stage while step 0 runs; W of turn
-    // `after` into the registers of steps 0 to 2 as soon as these are done; and, in step 1, W of turn `next` into the other set's
-    // step 3, which the turn before had used to its end.  X's operands are read three ahead.
-    auto products = [&](int d, const bf16_t* stage, bf16_t* other, int next, int after) {
-        const bf16_t* xb = stage + r * 128;
-        gr_bf16x8_t x[4];
-#pragma unroll
-        for (int q = 0; q < 3; ++q) x[q] = *reinterpret_cast<const gr_bf16x8_t*>(xb + (q % MT) * 2048 + ((4 * (q / MT) + g) ^ r) * 8);
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_nop 1");
-#pragma unroll
-        for (int q = 0; q < 4 * MT; ++q) {
-            const int s = q / MT, i = q % MT, ahead = q + 3;
-            if (ahead < 4 * MT) x[ahead % 4] = *reinterpret_cast<const gr_bf16x8_t*>(xb + (ahead % MT) * 2048 + ((4 * (ahead / MT) + g) ^ r) * 8);
-            gr_mfma2(acc[0][i], acc[1][i], w[d][s][0], w[d][s][1], x[q % 4]);
-            __builtin_amdgcn_sched_barrier(0);
-            if (s == 0) load_x(other, i, next);
-            else if (i < 4) load_w(d, s - 1, i, after);
-            else if (s == 1 && i < 8) load_w(1 - d, 3, i - 4, next);
-            __builtin_amdgcn_sched_barrier(0);
-            gr_mfma2(acc[2][i], acc[3][i], w[d][s][2], w[d][s][3], x[q % 4]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    // A turn issues X's loads before its 16 loads of W, and loads return in order: at most 16 under way means that X is there
-    auto turn = [&]() {
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-    };
-#pragma unroll
-    for (int i = 0; i < MT; ++i) load_x(stage0, i, 0);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) load_w(0, s, j, 0);
-    turn();
-#pragma unroll
-    for (int s = 0; s < 3; ++s)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) load_w(1, s, j, min(1, n - 1));
-    __builtin_amdgcn_sched_barrier(0);
-    // (the last turns ask for the last turn's operands again: loads that a branch skips would make the compiler count fewer under way)
-    int c = 0;
-    for (; c + 1 < n; c += 2) {
-        const int after = min(c + 2, n - 1);
-        products(0, stage0, stage1, c + 1, after);
-        turn();
-        products(1, stage1, stage0, after, min(c + 3, n - 1));
-        turn();
-    }
-    if (c < n) products(0, stage0, stage1, n - 1, n - 1);
-    gr_sums_settle();
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-}
+struct TallBf16 {
+    typedef gr_bf16x8_t operand_t;
+    typedef gr_f32x4_t sums_t;
+    static __device__ __forceinline__ void mfma2(sums_t& a, sums_t& b, operand_t w0, operand_t w1, operand_t x) { gr_mfma2(a, b, w0, w1, x); }
+};
 
 template <int MT, int EPI>
 __global__ __launch_bounds__(256, 1) void gemm_rows_tall_kernel(void* C, const bf16_t* X, const bf16_t* W, int M, int N, int K, int n_rows, int n_cols,
@@ -137,7 +65,7 @@ __global__ __launch_bounds__(256, 1) void gemm_rows_tall_kernel(void* C, const b
     const int s_row = wave * 4 + (lane >> 4);
     const int x_lane = (s_row * K + ((lane & 15) ^ s_row) * 8) * 2, x_at = (row0 * K + c0 * 128) * 2;
     gr_f32x4_t acc[4][MT];
-    gr_tall_turns<MT>(acc, wres, w_lane, w_at, w_turn, n, stage0, stage1, lane, [&](bf16_t* stage, int i, int c) {
+    gr_tall_turns<TallBf16, MT>(acc, wres, w_lane, w_at, w_turn, n, stage0, stage1, lane, [&](bf16_t* stage, int i, int c) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (__attribute__((address_space(3))) void*)(stage + (i * 4 + wave) * 512), 16, x_lane,
                                                  x_at + i * 32 * K + c * 256, 0, 0);
     });
