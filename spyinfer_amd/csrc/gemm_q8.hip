@@ -1,75 +1,253 @@
 // Products of 8-bit integer rows with 8-bit integer matrices (q8.h has both forms), sums in 32-bit integers, which hold them exactly
 // (K < 2^17):  y[m][n] = sum * row scale * column scale, rounded once; or the gated pair of such values.
+//
+// Few rows and some: a block has MT row tiles and NT column tiles (gated: the gate's and the up values' of the same columns).  Its waves take steps of 64 of K in
+// turn, each all of the block's tiles, so that every byte goes from memory into the registers of the one wave that multiplies it: nothing passes
+// through LDS before the waves' sums, which are added there at the end, and no wave waits for another until then.  A wave keeps D steps under way.
+// Steps behind the end are loads beyond their buffers: they ask the memory for nothing and bring zeros.
 #include "gemm_q8.h"
 
-#define Q8_WAVES 4
+// A tile of results: row tile i and column tile j of a block from (row0, 16 col0) on; lane 16 g + r has row r and columns 4 g ..
+template <int EPI, int NT, int NO, typename TC>
+__device__ __forceinline__ void q8_store_tile(TC* C, const q8_i32x4_t& sum, const q8_i32x4_t& up, int i, int j, int row0, int col0, int rows, int N, int r, int g,
+                                              const float* row_scales, const float* col_scales, const GateAct& act) {
+    const int n = (col0 + j) * 16 + 4 * g;
+    const float fx = row_scales[i * 16 + r];
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = q8_value<EPI>(act, sum[e], up[e], fx, col_scales[j * 16 + 4 * g + e], col_scales[(NT - NO + j) * 16 + 4 * g + e]);
+    if (i * 16 + r >= rows) return;
+    TC* o = C + (size_t)(row0 + i * 16 + r) * N + n;
+    if (N % 4 == 0 && (uintptr_t)C % (4 * sizeof(TC)) == 0) { if (n < N) Vec4<TC>::store(o, y); }
+    else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < N) o[e] = from_f32<TC>(y[e]);
+    }
+}
 
-// One block has 16 MT rows and one column tile (gated: the gate's and the up values' of the same columns); its waves share K by chunks
-// and add through LDS.
-template <int MT, int EPI, typename TC>
-__global__ __launch_bounds__(Q8_WAVES * 64) void gemm_q8_kernel(TC* __restrict__ C, const int8_t* __restrict__ X, int64_t pitch, const float* __restrict__ sx,
-                                                                const int8_t* __restrict__ W, const float* __restrict__ sw, int M, int N, int tiles, int chunks,
-                                                                GateAct act) {
-    constexpr int NT = EPI == Q8_GATED ? 2 : 1;
-    __shared__ q8_i32x4_t red[Q8_WAVES - 1][NT][MT][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int tile = blockIdx.x, row0 = blockIdx.y * MT * 16;
-    const int rows = min(M - row0, MT * 16);
-    // what lies behind the last row reads as zeros; behind a row's end the matrix has zeros
-    const auto xres = __builtin_amdgcn_make_buffer_rsrc((void*)(X + (size_t)row0 * pitch), 0, (int)(rows * pitch), 0x00020000);
-    q8_i32x4_t acc[NT][MT];
+template <int WAVES, int MT, int NT, int D, int EPI, typename TC>
+__global__ __launch_bounds__(WAVES * 64) void gemm_q8_kernel(TC* __restrict__ C, const int8_t* __restrict__ X, int64_t pitch, const float* __restrict__ sx,
+                                                             const int8_t* __restrict__ W, const float* __restrict__ sw, int M, int N, int tiles, int chunks,
+                                                             int n_rows, int blocks, GateAct act) {
+    constexpr int PAIR = EPI == Q8_GATED ? 2 : 1, NO = NT / PAIR;                   // column tiles of results
+    constexpr int ITEMS = MT * NO, MOST = 64 / (WAVES * PAIR), PHASE = ITEMS < MOST ? ITEMS : MOST;      // tiles of results added at a time: 64 KB
+    __shared__ q8_i32x4_t red[WAVES][PHASE][PAIR][64];
+    __shared__ float row_scales[MT * 16], col_scales[NT * 16];
+    const int per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;    // (a die takes a run of the blocks: gemm_q8_tall_kernel)
+    const int v = (blockIdx.x % Q8_DIES) * per + idx;
+    if (idx >= per || v >= blocks) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4, tid = threadIdx.x;
+    const int col0 = v / n_rows * NO, row0 = (v % n_rows) * MT * 16, rows = min(M - row0, MT * 16);
+    // the scales are asked for ahead of the rows: they are there when the sums are
+    static_assert(MT * 16 + NT * 16 <= WAVES * 64, "a thread for each scale");
+    float scale = 0.f;
+    if (tid < MT * 16) { if (tid < rows) scale = sx[row0 + tid]; }
+    else if (tid < (MT + NT) * 16) {
+        const int n = tid - MT * 16, tile = col0 + n / 16 % NO;
+        if (tile < tiles / PAIR) scale = sw[(n / 16 / NO * (tiles / PAIR) + tile) * 16 + n % 16];
+    }
+    const int w_bytes = tiles * chunks * 4096, x_bytes = (int)(rows * pitch), n_steps = chunks * 4;
+    const auto wres = __builtin_amdgcn_make_buffer_rsrc((void*)W, 0, w_bytes, 0x00020000);
+    const auto xres = __builtin_amdgcn_make_buffer_rsrc((void*)(X + row0 * pitch), 0, x_bytes, 0x00020000);
+    int w_at[NT], x_at[MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) w_at[j] = min(col0 + j % NO, tiles / PAIR - 1) * 4096 + j / NO * (tiles / PAIR) * 4096;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x_at[i] = (i * 16 + r) * (int)pitch + g * 16;
+    q8_i32x4_t acc[NT][MT], w[D][NT], x[D][MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = q8_i32x4_t{0, 0, 0, 0};
-    for (int c = wave; c < chunks; c += Q8_WAVES) {
+    auto load = [&](int d, int step) {
+        const bool some = step < n_steps;
+        const int wo = some ? (step >> 2) * tiles * 4096 + (step & 3) * 1024 : w_bytes, xo = some ? step * Q8_STEP : x_bytes;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            q8_i32x4_t w[NT];
+        for (int j = 0; j < NT; ++j) w[d][j] = __builtin_bit_cast(q8_i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(wres, lane * 16, w_at[j] + wo, 0));
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-                w[j] = *reinterpret_cast<const q8_i32x4_t*>(W + ((size_t)c * tiles + tile + j * (tiles / 2)) * 4096 + s * 1024 + lane * 16);
+        for (int i = 0; i < MT; ++i) x[d][i] = __builtin_bit_cast(q8_i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xres, x_at[i], xo, 0));
+    };
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int at = (i * 16 + r) * (int)pitch + c * Q8_CHUNK + s * Q8_STEP + g * 16;
-                const q8_i32x4_t x = __builtin_bit_cast(q8_i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xres, at, 0, 0));
+    for (int d = 0; d < D; ++d) load(d, wave + d * WAVES);
+    for (int s = wave; s < n_steps; s += D * WAVES) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[j][i] = q8_mfma(w[j], x, acc[j][i]);
-            }
+        for (int d = 0; d < D; ++d) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[j][i] = q8_mfma(w[d][j], x[d][i], acc[j][i]);
+            load(d, s + (D + d) * WAVES);
         }
     }
-    if (wave) {
+    if (tid < MT * 16) row_scales[tid] = scale;
+    else if (tid < (MT + NT) * 16) col_scales[tid - MT * 16] = scale;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+    for (int t0 = 0; t0 < ITEMS; t0 += PHASE) {
+        if (t0) __syncthreads();
 #pragma unroll
-            for (int i = 0; i < MT; ++i) red[wave - 1][j][i][lane] = acc[j][i];
-    }
-    __syncthreads();
-    if (wave) return;
+        for (int t = t0; t < t0 + PHASE && t < ITEMS; ++t)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+            for (int p = 0; p < PAIR; ++p) red[wave][t - t0][p][lane] = acc[p * NO + t % NO][t / NO];
+        __syncthreads();
+        for (int t = t0 + wave; t < min(t0 + PHASE, ITEMS); t += WAVES) {
+            q8_i32x4_t sum[PAIR];
 #pragma unroll
-        for (int v = 0; v < Q8_WAVES - 1; ++v)
+            for (int p = 0; p < PAIR; ++p) {
+                sum[p] = red[0][t - t0][p][lane];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[j][i] += red[v][j][i][lane];
-        const int m = row0 + i * 16 + r;
-        if (m >= M) continue;
-        const float fx = sx[m];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int n = tile * 16 + 4 * g + e;
-            if (n >= N) continue;
-            float y = (float)acc[0][i][e] * fx * sw[n];
-            if (EPI == Q8_GATED) y = gated_value_short(act, y, (float)acc[NT - 1][i][e] * fx * sw[n + tiles * 8]);
-            C[(size_t)m * N + n] = from_f32<TC>(y);
+                for (int u = 1; u < WAVES; ++u) sum[p] += red[u][t - t0][p][lane];
+            }
+            q8_store_tile<EPI, NT, NO>(C, sum[0], sum[PAIR - 1], t / NO, t % NO, row0, col0, rows, N, r, g, row_scales, col_scales, act);
         }
     }
 }
 
+// waits until at most N loads are under way (and for nothing else)
+template <int N>
+__device__ __forceinline__ void q8_wait_loads() {
+    static_assert(N >= 0 && N <= 63, "the counter has six bits");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
+    asm volatile("" ::: "memory");
+}
+
+// The same with X through LDS, in a part that a wave has to itself: a wave's loads of X into LDS bring whole pieces of 64 S bytes of a row (an operand of 16
+// rows straight from memory is 64 pieces of 16 bytes, which take the address unit 64 clocks a KB), and its reads from there are the operands.  A wave's
+// unit is S steps, D units are under way.  Piece p of row r of a tile lies at place p ^ (r S / 4), so that the reads meet in no bank.
+template <int WAVES, int MT, int NT, int S, int D, int EPI, typename TC>
+__device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks,
+                                                int n_rows, int blocks, const GateAct& act) {
+    constexpr int PAIR = EPI == Q8_GATED ? 2 : 1, NO = NT / PAIR, PIECES = 4 * S, RPI = 16 / S;            // pieces of a row, rows that a load brings
+    constexpr int ITEMS = MT * NO, MOST = MT * S / PAIR, PHASE = ITEMS < MOST ? ITEMS : MOST, OPS = MT * S + NT * S;
+    static_assert(D >= 2 && D <= 3 && (D - 1) * OPS <= 63, "a wait counts the loads issued after those that it waits for");
+    // (arrays of their own: reads of one that the compiler cannot tell from another would wait for that one's loads)
+    __shared__ __align__(1024) char stage0[WAVES * MT * S * 1024];
+    __shared__ __align__(1024) char stage1[WAVES * MT * S * 1024];
+    __shared__ __align__(1024) char stage2[D > 2 ? WAVES * MT * S * 1024 : 16];
+    __shared__ float row_scales[MT * 16], col_scales[NT * 16];
+    const int per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;    // (a die takes a run of the blocks: gemm_q8_tall_kernel)
+    const int v = (blockIdx.x % Q8_DIES) * per + idx;
+    if (idx >= per || v >= blocks) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4, tid = threadIdx.x;
+    const int col0 = v / n_rows * NO, row0 = (v % n_rows) * MT * 16, rows = min(M - row0, MT * 16);
+    static_assert(MT * 16 + NT * 16 <= WAVES * 64, "a thread for each scale");
+    float scale = 0.f;
+    if (tid < MT * 16) { if (tid < rows) scale = sx[row0 + tid]; }
+    else if (tid < (MT + NT) * 16) {
+        const int n = tid - MT * 16, tile = col0 + n / 16 % NO;
+        if (tile < tiles / PAIR) scale = sw[(n / 16 / NO * (tiles / PAIR) + tile) * 16 + n % 16];
+    }
+    const int w_bytes = tiles * chunks * 4096, x_bytes = (int)(rows * pitch), n_units = chunks * 4 / S;
+    const auto wres = __builtin_amdgcn_make_buffer_rsrc((void*)W, 0, w_bytes, 0x00020000);
+    const auto xres = __builtin_amdgcn_make_buffer_rsrc((void*)(X + row0 * pitch), 0, x_bytes, 0x00020000);
+    int w_at[NT], x_lane[S];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) w_at[j] = min(col0 + j % NO, tiles / PAIR - 1) * 4096 + j / NO * (tiles / PAIR) * 4096;
+#pragma unroll
+    for (int q = 0; q < S; ++q) x_lane[q] = (q * RPI + lane / PIECES) * (int)pitch + (lane % PIECES ^ (q * RPI + lane / PIECES) * S / 4) * 16;
+    q8_i32x4_t acc[NT][MT], w[D][S][NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = q8_i32x4_t{0, 0, 0, 0};
+    char* const mine[3] = {stage0 + wave * MT * S * 1024, stage1 + wave * MT * S * 1024, stage2 + (D > 2 ? wave * MT * S * 1024 : 0)};
+    auto load = [&](int d, int unit) {
+        const bool some = unit < n_units;
+        const int wo = some ? (unit * S >> 2) * tiles * 4096 + (unit * S & 3) * 1024 : w_bytes, xo = some ? unit * S * Q8_STEP : x_bytes;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int q = 0; q < S; ++q)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (__attribute__((address_space(3))) void*)(mine[d] + (i * S + q) * 1024), 16, x_lane[q], xo + i * 16 * (int)pitch, 0, 0);
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) w[d][s][j] = __builtin_bit_cast(q8_i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(wres, lane * 16, w_at[j] + wo + s * 1024, 0));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(d, wave + d * WAVES);
+    for (int u = wave; u < n_units; u += D * WAVES) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            // loads return in order: those of the D - 1 units behind this one may be under way
+            __builtin_amdgcn_sched_barrier(0);
+            q8_wait_loads<(D - 1) * OPS>();
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                q8_i32x4_t x[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) x[i] = *reinterpret_cast<const q8_i32x4_t*>(mine[d] + (i * 16 + r) * 64 * S + ((4 * s + g) ^ r * S / 4) * 16);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[j][i] = q8_mfma(w[d][s][j], x[i], acc[j][i]);
+            }
+            __builtin_amdgcn_sched_barrier(0);       // (the stage has been read: the products wait for the reads)
+            load(d, u + (D + d) * WAVES);
+        }
+    }
+    if (tid < MT * 16) row_scales[tid] = scale;
+    else if (tid < (MT + NT) * 16) col_scales[tid - MT * 16] = scale;
+    // nothing is under way into the stages when the sums go there
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    q8_i32x4_t* const red = reinterpret_cast<q8_i32x4_t*>(stage0);          // [WAVES][PHASE][PAIR][64]
+#pragma unroll
+    for (int t0 = 0; t0 < ITEMS; t0 += PHASE) {
+        __syncthreads();
+#pragma unroll
+        for (int t = t0; t < t0 + PHASE && t < ITEMS; ++t)
+#pragma unroll
+            for (int p = 0; p < PAIR; ++p) red[((wave * PHASE + t - t0) * PAIR + p) * 64 + lane] = acc[p * NO + t % NO][t / NO];
+        __syncthreads();
+        for (int t = t0 + wave; t < min(t0 + PHASE, ITEMS); t += WAVES) {
+            q8_i32x4_t sum[PAIR];
+#pragma unroll
+            for (int p = 0; p < PAIR; ++p) {
+                sum[p] = red[((t - t0) * PAIR + p) * 64 + lane];
+#pragma unroll
+                for (int u = 1; u < WAVES; ++u) sum[p] += red[((u * PHASE + t - t0) * PAIR + p) * 64 + lane];
+            }
+            q8_store_tile<EPI, NT, NO>(C, sum[0], sum[PAIR - 1], t / NO, t % NO, row0, col0, rows, N, r, g, row_scales, col_scales, act);
+        }
+    }
+}
+
+template <int WAVES, int MT, int NT, int S, int D, int EPI, typename TC>
+__global__ __launch_bounds__(WAVES * 64) void gemm_q8_staged_kernel(TC* C, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N,
+                                                                    int tiles, int chunks, int n_rows, int blocks, GateAct act) {
+    q8_staged_block<WAVES, MT, NT, S, D, EPI, TC>(C, X, pitch, sx, W, sw, M, N, tiles, chunks, n_rows, blocks, act);
+}
+
+struct Q8Args {
+    void* C; int c_dtype; const int8_t* X; int64_t pitch; const float* sx; const int8_t* W; const float* sw; int M, N, tiles, chunks, gated; GateAct act; hipStream_t st;
+};
+
+template <int WAVES, int MT, int NT, int S, int D>
+static int split_launch(const Q8Args& a) {
+    const int no = a.gated ? NT / 2 : NT, col_tiles = a.gated ? a.tiles / 2 : a.tiles;
+    const int n_rows = (a.M + MT * 16 - 1) / (MT * 16), n_cols = (col_tiles + no - 1) / no;
+    const int64_t blocks = (int64_t)n_rows * n_cols;
+    SPY_REQUIRE(blocks < (1 << 30), "spy_gemm_q8: %lld blocks", (long long)blocks);
+    const unsigned grid = (unsigned)((blocks + Q8_DIES - 1) / Q8_DIES * Q8_DIES);
+#define SPLIT_ARGS(TC) (TC*)a.C, a.X, a.pitch, a.sx, a.W, a.sw, a.M, a.N, a.tiles, a.chunks, n_rows, (int)blocks, a.act
+#define SPLIT(EPI, TC) do { if constexpr (S == 0) gemm_q8_kernel<WAVES, MT, NT, D, EPI, TC><<<grid, WAVES * 64, 0, a.st>>>(SPLIT_ARGS(TC)); \
+                            else gemm_q8_staged_kernel<WAVES, MT, NT, S, D, EPI, TC><<<grid, WAVES * 64, 0, a.st>>>(SPLIT_ARGS(TC)); } while (0)
+    if (a.gated) { if constexpr (NT % 2 == 0) SPLIT(Q8_GATED, bf16_t); else return spy_fail("spy_gemm_q8: a gated product by %d column tiles", NT); }
+    else if (a.c_dtype == SPY_F32) SPLIT(Q8_STORE, float);
+    else SPLIT(Q8_STORE, bf16_t);
+#undef SPLIT
+#undef SPLIT_ARGS
+    SPY_CHECK_LAUNCH("spy_gemm_q8");
+    return 0;
+}
+
 // C: bfloat16 or float32 [M, N].  X: rows of `pitch` bytes (a multiple of 16) and their scales; W: the matrix laid out, `tiles` column tiles (gated:
 // of both halves) and `chunks` of K, and its scales [16 tiles].  Gated: C is bfloat16 [M, N], N one half's columns.
+// plan: 0, or the blocks by name: 8 to 16 row tiles (tall), or 100 NT + MT.
 extern "C" int spy_gemm_q8(void* C, int c_dtype, const void* X, int64_t pitch, const float* sx, const void* W, const float* sw, int M, int N, int tiles, int chunks,
-                           int gated, int act_code, hipStream_t st) {
+                           int gated, int act_code, int plan, hipStream_t st) {
     GateAct act = {1.f, 0.f};
     SPY_REQUIRE(M > 0 && N > 0 && tiles > 0 && chunks > 0, "spy_gemm_q8: empty operand");
     SPY_REQUIRE(pitch % 16 == 0 && pitch <= (int64_t)chunks * Q8_CHUNK && pitch > (int64_t)(chunks - 1) * Q8_CHUNK, "spy_gemm_q8: rows of %lld bytes for %d chunks of K", (long long)pitch, chunks);
@@ -77,14 +255,30 @@ extern "C" int spy_gemm_q8(void* C, int c_dtype, const void* X, int64_t pitch, c
     SPY_REQUIRE(gated ? tiles % 2 == 0 && N <= tiles * 8 && N > tiles * 8 - 16 : N <= tiles * 16 && N > tiles * 16 - 16, "spy_gemm_q8: %d columns in %d tiles", N, tiles);
     SPY_REQUIRE((((uintptr_t)X | (uintptr_t)W) % 16) == 0, "spy_gemm_q8: operands must be 16-byte aligned");
     SPY_REQUIRE(!gated || (gate_act_of(act_code, &act) && c_dtype == SPY_BF16), "spy_gemm_q8: activation %d, result dtype %d", act_code, c_dtype);
-    SPY_REQUIRE(M <= 65535 * 64, "spy_gemm_q8: too many rows");
-    if (M > 512) return q8_tall_launch(C, c_dtype, (const int8_t*)X, pitch, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, 16, st);
-#define Q8(MT, EPI, TC) gemm_q8_kernel<MT, EPI, TC><<<dim3(EPI == Q8_GATED ? tiles / 2 : tiles, (M + 16 * MT - 1) / (16 * MT)), Q8_WAVES * 64, 0, st>>>( \
-        (TC*)C, (const int8_t*)X, pitch, sx, (const int8_t*)W, sw, M, N, tiles, chunks, act)
-    if (gated) { if (M <= 16) Q8(1, Q8_GATED, bf16_t); else Q8(4, Q8_GATED, bf16_t); }
-    else if (c_dtype == SPY_F32) { if (M <= 16) Q8(1, Q8_STORE, float); else Q8(4, Q8_STORE, float); }
-    else { if (M <= 16) Q8(1, Q8_STORE, bf16_t); else Q8(4, Q8_STORE, bf16_t); }
-#undef Q8
-    SPY_CHECK_LAUNCH("spy_gemm_q8");
-    return 0;
+    const Q8Args a = {C, c_dtype, (const int8_t*)X, pitch, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, st};
+    if (!plan) plan = M <= 16 ? (gated ? 201 : 101) : M <= 64 ? 1200 + (M + 15) / 16 : M <= 512 ? 1400 + (M <= 128 ? (M + 15) / 16 : 8) : 16;
+    if (plan >= 8 && plan <= 16) return q8_tall_launch(C, c_dtype, (const int8_t*)X, pitch, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, plan, st);
+    switch (plan) {
+        case 101: return split_launch<8, 1, 1, 0, 8>(a);
+        case 201: return split_launch<8, 1, 2, 0, 6>(a);
+        case 1101: return split_launch<8, 1, 1, 4, 2>(a);
+        case 1102: return split_launch<8, 2, 1, 2, 3>(a);
+        case 1103: return split_launch<8, 3, 1, 2, 2>(a);
+        case 1104: return split_launch<8, 4, 1, 2, 2>(a);
+        case 1201: return split_launch<8, 1, 2, 4, 2>(a);
+        case 1202: return split_launch<8, 2, 2, 2, 2>(a);
+        case 1203: return split_launch<8, 3, 2, 2, 2>(a);
+        case 1204: return split_launch<8, 4, 2, 2, 2>(a);
+        case 1402: return split_launch<4, 2, 4, 2, 3>(a);
+        case 1403: return split_launch<4, 3, 4, 2, 2>(a);
+        case 1404: return split_launch<4, 4, 4, 2, 2>(a);
+        case 1405: return split_launch<4, 5, 4, 2, 2>(a);
+        case 1406: return split_launch<4, 6, 4, 2, 2>(a);
+        case 1407: return split_launch<4, 7, 4, 2, 2>(a);
+        case 1408: return split_launch<4, 8, 4, 2, 2>(a);
+        case 2404: return split_launch<8, 4, 4, 2, 2>(a);
+        case 2406: return split_launch<8, 6, 4, 1, 2>(a);
+        case 2408: return split_launch<8, 8, 4, 1, 2>(a);
+    }
+    return spy_fail("spy_gemm_q8: no blocks by the name of %d", plan);
 }

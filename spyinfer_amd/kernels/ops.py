@@ -94,7 +94,7 @@ class _Hip:
         # ctypes object per argument: 3 us of the host's 14 per call)
         P, I = ctypes.c_void_p, ctypes.c_int
         self.lib.spy_gemm_decode.argtypes = [P, I, P, I, ctypes.c_float, P, I, P, I, P, P, P, P, I, I, I, I, I, I, P, ctypes.c_int64, I, P]
-        self.lib.spy_gemm_q8.argtypes = [P, I, P, ctypes.c_int64, P, P, P, I, I, I, I, I, I, P]
+        self.lib.spy_gemm_q8.argtypes = [P, I, P, ctypes.c_int64, P, P, P, I, I, I, I, I, I, I, P]
         self.lib.spy_add_rmsnorm_q8.argtypes = [P, P, P, P, I, P, I, ctypes.c_float, I, I, ctypes.c_int64, P]
         self.lib.spy_quantize_rows.argtypes = [P, P, P, I, ctypes.c_int64, I, I, ctypes.c_int64, P]
 
@@ -2736,6 +2736,8 @@ def moe_experts(x: torch.Tensor, ids: Optional[torch.Tensor], weights: Optional[
 
 #: widest rows of a product in 8-bit integers: its sums stay within 32 bits
 Q8_MAX_WIDTH = 511 * 256
+#: 0: the kernels' own rule; else the blocks of the next products by name (csrc/gemm_q8.hip), for tests of every kind of block
+Q8_PLAN = 0
 
 
 def _q8_pitch(width: int) -> int:
@@ -2867,7 +2869,7 @@ def _gemm_q8(x: Q8Rows, w: Q8Weight, out: torch.Tensor, columns: int, act: int) 
     if out.shape[0]:
         with _on_device_of(out):
             hip().call("spy_gemm_q8", out.data_ptr(), _CODES[out.dtype], x.values.data_ptr(), x.values.shape[1], x.scales.data_ptr(), w.tiles.data_ptr(),
-                       w.scales.data_ptr(), out.shape[0], columns, w.tiles.shape[1], w.tiles.shape[0], 1 if w.gated else 0, act, _Hip.stream())
+                       w.scales.data_ptr(), out.shape[0], columns, w.tiles.shape[1], w.tiles.shape[0], 1 if w.gated else 0, act, Q8_PLAN, _Hip.stream())
     return out
 
 
