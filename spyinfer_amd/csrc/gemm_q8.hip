@@ -1,10 +1,13 @@
 // Products of 8-bit integer rows with 8-bit integer matrices (q8.h has both forms), sums in 32-bit integers, which hold them exactly
 // (K < 2^17):  y[m][n] = sum * row scale * column scale, rounded once; or the gated pair of such values.
 //
-// Few rows and some: a block has MT row tiles and NT column tiles (gated: the gate's and the up values' of the same columns).  Its waves take steps of 64 of K in
-// turn, each all of the block's tiles, so that every byte goes from memory into the registers of the one wave that multiplies it: nothing passes
-// through LDS before the waves' sums, which are added there at the end, and no wave waits for another until then.  A wave keeps D steps under way.
-// Steps behind the end are loads beyond their buffers: they ask the memory for nothing and bring zeros.
+// Few rows and some: a block has MT row tiles and NT column tiles (gated: the gate's and the up values' of the same columns).  Its four waves take units
+// of S steps of 64 of K in turn, each all of the block's tiles, so that every byte is loaded by the one wave that multiplies it, and no wave
+// waits for another before their sums are added, through LDS, at the end.  W goes from memory into operand registers, a kilobyte a load.  X goes through LDS, in a part that a
+// wave has to itself: its loads there bring whole pieces of 64 S bytes of a row, its reads from there are the operands (16 rows straight from memory
+// are 64 pieces of 16 bytes a load, which take the address unit 64 clocks: 64 rows, 12288 -> 4096 30.6 us for 20.7).  Piece p of row r of a tile
+// lies at place p ^ (r S / 4), so that the reads meet in no bank.  A wave keeps D units under way; units behind the end are loads beyond their buffers, which ask
+// the memory for nothing and bring zeros.
 #include "gemm_q8.h"
 
 // A tile of results: row tile i and column tile j of a block from (row0, 16 col0) on; lane 16 g + r has row r and columns 4 g ..
@@ -26,83 +29,6 @@ __device__ __forceinline__ void q8_store_tile(TC* C, const q8_i32x4_t& sum, cons
     }
 }
 
-template <int WAVES, int MT, int NT, int D, int EPI, typename TC>
-__global__ __launch_bounds__(WAVES * 64) void gemm_q8_kernel(TC* __restrict__ C, const int8_t* __restrict__ X, int64_t pitch, const float* __restrict__ sx,
-                                                             const int8_t* __restrict__ W, const float* __restrict__ sw, int M, int N, int tiles, int chunks,
-                                                             int n_rows, int blocks, GateAct act) {
-    constexpr int PAIR = EPI == Q8_GATED ? 2 : 1, NO = NT / PAIR;                   // column tiles of results
-    constexpr int ITEMS = MT * NO, MOST = 64 / (WAVES * PAIR), PHASE = ITEMS < MOST ? ITEMS : MOST;      // tiles of results added at a time: 64 KB
-    __shared__ q8_i32x4_t red[WAVES][PHASE][PAIR][64];
-    __shared__ float row_scales[MT * 16], col_scales[NT * 16];
-    const int per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;    // (a die takes a run of the blocks: gemm_q8_tall_kernel)
-    const int v = (blockIdx.x % Q8_DIES) * per + idx;
-    if (idx >= per || v >= blocks) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4, tid = threadIdx.x;
-    const int col0 = v / n_rows * NO, row0 = (v % n_rows) * MT * 16, rows = min(M - row0, MT * 16);
-    // the scales are asked for ahead of the rows: they are there when the sums are
-    static_assert(MT * 16 + NT * 16 <= WAVES * 64, "a thread for each scale");
-    float scale = 0.f;
-    if (tid < MT * 16) { if (tid < rows) scale = sx[row0 + tid]; }
-    else if (tid < (MT + NT) * 16) {
-        const int n = tid - MT * 16, tile = col0 + n / 16 % NO;
-        if (tile < tiles / PAIR) scale = sw[(n / 16 / NO * (tiles / PAIR) + tile) * 16 + n % 16];
-    }
-    const int w_bytes = tiles * chunks * 4096, x_bytes = (int)(rows * pitch), n_steps = chunks * 4;
-    const auto wres = __builtin_amdgcn_make_buffer_rsrc((void*)W, 0, w_bytes, 0x00020000);
-    const auto xres = __builtin_amdgcn_make_buffer_rsrc((void*)(X + row0 * pitch), 0, x_bytes, 0x00020000);
-    int w_at[NT], x_at[MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) w_at[j] = min(col0 + j % NO, tiles / PAIR - 1) * 4096 + j / NO * (tiles / PAIR) * 4096;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) x_at[i] = (i * 16 + r) * (int)pitch + g * 16;
-    q8_i32x4_t acc[NT][MT], w[D][NT], x[D][MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[j][i] = q8_i32x4_t{0, 0, 0, 0};
-    auto load = [&](int d, int step) {
-        const bool some = step < n_steps;
-        const int wo = some ? (step >> 2) * tiles * 4096 + (step & 3) * 1024 : w_bytes, xo = some ? step * Q8_STEP : x_bytes;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) w[d][j] = __builtin_bit_cast(q8_i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(wres, lane * 16, w_at[j] + wo, 0));
-#pragma unroll
-        for (int i = 0; i < MT; ++i) x[d][i] = __builtin_bit_cast(q8_i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xres, x_at[i], xo, 0));
-    };
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(d, wave + d * WAVES);
-    for (int s = wave; s < n_steps; s += D * WAVES) {
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[j][i] = q8_mfma(w[d][j], x[d][i], acc[j][i]);
-            load(d, s + (D + d) * WAVES);
-        }
-    }
-    if (tid < MT * 16) row_scales[tid] = scale;
-    else if (tid < (MT + NT) * 16) col_scales[tid - MT * 16] = scale;
-#pragma unroll
-    for (int t0 = 0; t0 < ITEMS; t0 += PHASE) {
-        if (t0) __syncthreads();
-#pragma unroll
-        for (int t = t0; t < t0 + PHASE && t < ITEMS; ++t)
-#pragma unroll
-            for (int p = 0; p < PAIR; ++p) red[wave][t - t0][p][lane] = acc[p * NO + t % NO][t / NO];
-        __syncthreads();
-        for (int t = t0 + wave; t < min(t0 + PHASE, ITEMS); t += WAVES) {
-            q8_i32x4_t sum[PAIR];
-#pragma unroll
-            for (int p = 0; p < PAIR; ++p) {
-                sum[p] = red[0][t - t0][p][lane];
-#pragma unroll
-                for (int u = 1; u < WAVES; ++u) sum[p] += red[u][t - t0][p][lane];
-            }
-            q8_store_tile<EPI, NT, NO>(C, sum[0], sum[PAIR - 1], t / NO, t % NO, row0, col0, rows, N, r, g, row_scales, col_scales, act);
-        }
-    }
-}
-
 // waits until at most N loads are under way (and for nothing else)
 template <int N>
 __device__ __forceinline__ void q8_wait_loads() {
@@ -111,10 +37,8 @@ __device__ __forceinline__ void q8_wait_loads() {
     asm volatile("" ::: "memory");
 }
 
-// The same with X through LDS, in a part that a wave has to itself: a wave's loads of X into LDS bring whole pieces of 64 S bytes of a row (an operand of 16
-// rows straight from memory is 64 pieces of 16 bytes, which take the address unit 64 clocks a KB), and its reads from there are the operands.  A wave's
-// unit is S steps, D units are under way.  Piece p of row r of a tile lies at place p ^ (r S / 4), so that the reads meet in no bank.
-template <int WAVES, int MT, int NT, int S, int D, int EPI, typename TC>
+// ONCE: W is read by one block only, and passes the caches by (up to 64 rows, matrices from memory: 16 rows, 4096 -> 2 x 12288 19.8 / 18.4 us).
+template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename TC>
 __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks,
                                                 int n_rows, int blocks, const GateAct& act) {
     constexpr int PAIR = EPI == Q8_GATED ? 2 : 1, NO = NT / PAIR, PIECES = 4 * S, RPI = 16 / S;            // pieces of a row, rows that a load brings
@@ -162,7 +86,7 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, int64_t 
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) w[d][s][j] = __builtin_bit_cast(q8_i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(wres, lane * 16, w_at[j] + wo + s * 1024, 0));
+            for (int j = 0; j < NT; ++j) w[d][s][j] = __builtin_bit_cast(q8_i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(wres, lane * 16, w_at[j] + wo + s * 1024, ONCE ? 2 : 0));
         __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
@@ -214,17 +138,17 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, int64_t 
     }
 }
 
-template <int WAVES, int MT, int NT, int S, int D, int EPI, typename TC>
-__global__ __launch_bounds__(WAVES * 64) void gemm_q8_staged_kernel(TC* C, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N,
+template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename TC>
+__global__ __launch_bounds__(WAVES * 64) void gemm_q8_kernel(TC* C, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N,
                                                                     int tiles, int chunks, int n_rows, int blocks, GateAct act) {
-    q8_staged_block<WAVES, MT, NT, S, D, EPI, TC>(C, X, pitch, sx, W, sw, M, N, tiles, chunks, n_rows, blocks, act);
+    q8_staged_block<WAVES, MT, NT, S, D, ONCE, EPI, TC>(C, X, pitch, sx, W, sw, M, N, tiles, chunks, n_rows, blocks, act);
 }
 
 struct Q8Args {
     void* C; int c_dtype; const int8_t* X; int64_t pitch; const float* sx; const int8_t* W; const float* sw; int M, N, tiles, chunks, gated; GateAct act; hipStream_t st;
 };
 
-template <int WAVES, int MT, int NT, int S, int D>
+template <int MT, int NT, int S, int D>
 static int split_launch(const Q8Args& a) {
     const int no = a.gated ? NT / 2 : NT, col_tiles = a.gated ? a.tiles / 2 : a.tiles;
     const int n_rows = (a.M + MT * 16 - 1) / (MT * 16), n_cols = (col_tiles + no - 1) / no;
@@ -232,20 +156,53 @@ static int split_launch(const Q8Args& a) {
     SPY_REQUIRE(blocks < (1 << 30), "spy_gemm_q8: %lld blocks", (long long)blocks);
     const unsigned grid = (unsigned)((blocks + Q8_DIES - 1) / Q8_DIES * Q8_DIES);
 #define SPLIT_ARGS(TC) (TC*)a.C, a.X, a.pitch, a.sx, a.W, a.sw, a.M, a.N, a.tiles, a.chunks, n_rows, (int)blocks, a.act
-#define SPLIT(EPI, TC) do { if constexpr (S == 0) gemm_q8_kernel<WAVES, MT, NT, D, EPI, TC><<<grid, WAVES * 64, 0, a.st>>>(SPLIT_ARGS(TC)); \
-                            else gemm_q8_staged_kernel<WAVES, MT, NT, S, D, EPI, TC><<<grid, WAVES * 64, 0, a.st>>>(SPLIT_ARGS(TC)); } while (0)
+#define SPLIT_BY(ONCE, EPI, TC) gemm_q8_kernel<4, MT, NT, S, D, ONCE, EPI, TC><<<grid, 256, 0, a.st>>>(SPLIT_ARGS(TC))
+    // (more than four row tiles, or four column tiles, are for products of more rows)
+#define SPLIT(EPI, TC) do { if (n_rows == 1 && MT <= 4 && NT <= 2) SPLIT_BY((MT <= 4 && NT <= 2), EPI, TC); else SPLIT_BY(false, EPI, TC); } while (0)
     if (a.gated) { if constexpr (NT % 2 == 0) SPLIT(Q8_GATED, bf16_t); else return spy_fail("spy_gemm_q8: a gated product by %d column tiles", NT); }
     else if (a.c_dtype == SPY_F32) SPLIT(Q8_STORE, float);
     else SPLIT(Q8_STORE, bf16_t);
 #undef SPLIT
+#undef SPLIT_BY
 #undef SPLIT_ARGS
     SPY_CHECK_LAUNCH("spy_gemm_q8");
     return 0;
 }
 
+// Which blocks: those with the least estimated time, us, of c[0] + c[1] r k + c[2] r + c[3] b k + c[4] x, b the blocks over 256 compute units, r that rounded up,
+// k the chunks of K; x: chunks of K that row tiles bring over the units, x k (tall blocks: b).  Fitted to 2720 products of 1 to 4096 rows, 256 to 34816 columns and K of 512 to 17408,
+// plain and gated, each with the matrices from memory, in every kind of block (4 to 13 % rms); what it takes is 1.3 % slower on average than the
+// fastest of all kinds, 7.5 % at the 95th percentile.  NT 100 + MT, or, tall, the row tiles alone.
+struct Q8Cost { int plan; float c[5]; };
+static const Q8Cost q8_costs[] = {
+    {101, {2.48f, 0.0793f, 0.627f, 0.f, 0.0674f}}, {102, {2.43f, 0.117f, 0.859f, 0.f, 0.0457f}}, {103, {2.37f, 0.154f, 1.19f, 0.f, 0.0351f}},
+    {104, {1.87f, 0.169f, 2.04f, 0.0456f, 0.00598f}}, {201, {2.44f, 0.141f, 0.504f, 0.149f, 0.f}}, {202, {2.44f, 0.168f, 0.741f, 0.0611f, 0.0554f}},
+    {203, {2.54f, 0.203f, 0.927f, 0.0379f, 0.0502f}}, {204, {2.8f, 0.218f, 1.06f, 0.0824f, 0.f}}, {206, {1.64f, 0.248f, 2.78f, 0.f, 0.0279f}},
+    {404, {3.43f, 0.277f, 1.45f, 0.192f, 0.f}}, {406, {1.55f, 0.363f, 4.58f, 0.f, 0.0354f}}, {408, {1.84f, 0.464f, 5.66f, 0.f, 0.0248f}},
+    {8, {2.26f, 1.08f, 3.97f, 0.584f, 3.25f}}, {10, {1.96f, 1.28f, 5.09f, 0.512f, 4.28f}}, {12, {1.61f, 1.44f, 6.05f, 0.579f, 4.88f}},
+    {14, {0.833f, 1.65f, 7.43f, 0.625f, 5.73f}}, {16, {0.011f, 1.88f, 8.71f, 0.647f, 6.44f}},
+};
+
+static int q8_plan(int M, int tiles, int chunks, int gated) {
+    const int row_tiles = (M + 15) / 16, col_tiles = gated ? tiles / 2 : tiles;
+    int best = 0;
+    float least = INFINITY;
+    for (const Q8Cost& p : q8_costs) {
+        const bool tall = p.plan < 100;
+        const int MT = tall ? p.plan : p.plan % 100, NO = tall ? (gated ? 8 : 16) : p.plan / 100 / (gated ? 2 : 1);
+        // up to three row tiles: as many as there are; more: not many more than there are (four from 33 rows on, six from 81, eight from 113, tall from 65)
+        if (NO < 1 || (tall ? M <= 64 : MT < 4 ? row_tiles != MT : MT == 4 ? row_tiles < 3 : row_tiles < MT)) continue;
+        const int cols = (col_tiles + NO - 1) / NO;
+        const float blocks = (float)((row_tiles + MT - 1) / MT) * (float)cols / 256.f, rounds = ceilf(blocks), k = (float)chunks;
+        const float us = p.c[0] + p.c[1] * rounds * k + p.c[2] * rounds + p.c[3] * blocks * k + p.c[4] * (tall ? blocks : (float)row_tiles * cols / 256.f * k);
+        if (us < least) { least = us; best = p.plan; }
+    }
+    return best;
+}
+
 // C: bfloat16 or float32 [M, N].  X: rows of `pitch` bytes (a multiple of 16) and their scales; W: the matrix laid out, `tiles` column tiles (gated:
 // of both halves) and `chunks` of K, and its scales [16 tiles].  Gated: C is bfloat16 [M, N], N one half's columns.
-// plan: 0, or the blocks by name: 8 to 16 row tiles (tall), or 100 NT + MT.
+// plan: 0, or the blocks by name (q8_costs).
 extern "C" int spy_gemm_q8(void* C, int c_dtype, const void* X, int64_t pitch, const float* sx, const void* W, const float* sw, int M, int N, int tiles, int chunks,
                            int gated, int act_code, int plan, hipStream_t st) {
     GateAct act = {1.f, 0.f};
@@ -256,29 +213,21 @@ extern "C" int spy_gemm_q8(void* C, int c_dtype, const void* X, int64_t pitch, c
     SPY_REQUIRE((((uintptr_t)X | (uintptr_t)W) % 16) == 0, "spy_gemm_q8: operands must be 16-byte aligned");
     SPY_REQUIRE(!gated || (gate_act_of(act_code, &act) && c_dtype == SPY_BF16), "spy_gemm_q8: activation %d, result dtype %d", act_code, c_dtype);
     const Q8Args a = {C, c_dtype, (const int8_t*)X, pitch, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, st};
-    if (!plan) plan = M <= 16 ? (gated ? 201 : 101) : M <= 64 ? 1200 + (M + 15) / 16 : M <= 512 ? 1400 + (M <= 128 ? (M + 15) / 16 : 8) : 16;
+    if (!plan) plan = q8_plan(M, tiles, chunks, gated);
     if (plan >= 8 && plan <= 16) return q8_tall_launch(C, c_dtype, (const int8_t*)X, pitch, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, plan, st);
     switch (plan) {
-        case 101: return split_launch<8, 1, 1, 0, 8>(a);
-        case 201: return split_launch<8, 1, 2, 0, 6>(a);
-        case 1101: return split_launch<8, 1, 1, 4, 2>(a);
-        case 1102: return split_launch<8, 2, 1, 2, 3>(a);
-        case 1103: return split_launch<8, 3, 1, 2, 2>(a);
-        case 1104: return split_launch<8, 4, 1, 2, 2>(a);
-        case 1201: return split_launch<8, 1, 2, 4, 2>(a);
-        case 1202: return split_launch<8, 2, 2, 2, 2>(a);
-        case 1203: return split_launch<8, 3, 2, 2, 2>(a);
-        case 1204: return split_launch<8, 4, 2, 2, 2>(a);
-        case 1402: return split_launch<4, 2, 4, 2, 3>(a);
-        case 1403: return split_launch<4, 3, 4, 2, 2>(a);
-        case 1404: return split_launch<4, 4, 4, 2, 2>(a);
-        case 1405: return split_launch<4, 5, 4, 2, 2>(a);
-        case 1406: return split_launch<4, 6, 4, 2, 2>(a);
-        case 1407: return split_launch<4, 7, 4, 2, 2>(a);
-        case 1408: return split_launch<4, 8, 4, 2, 2>(a);
-        case 2404: return split_launch<8, 4, 4, 2, 2>(a);
-        case 2406: return split_launch<8, 6, 4, 1, 2>(a);
-        case 2408: return split_launch<8, 8, 4, 1, 2>(a);
+        case 101: return split_launch<1, 1, 4, 2>(a);
+        case 102: return split_launch<2, 1, 2, 3>(a);
+        case 103: return split_launch<3, 1, 2, 3>(a);
+        case 104: return split_launch<4, 1, 2, 3>(a);
+        case 201: return split_launch<1, 2, 2, 2>(a);
+        case 202: return split_launch<2, 2, 2, 2>(a);
+        case 203: return split_launch<3, 2, 2, 2>(a);
+        case 204: return split_launch<4, 2, 2, 2>(a);
+        case 206: return split_launch<6, 2, 2, 2>(a);
+        case 404: return split_launch<4, 4, 2, 2>(a);
+        case 406: return split_launch<6, 4, 2, 2>(a);
+        case 408: return split_launch<8, 4, 2, 2>(a);
     }
     return spy_fail("spy_gemm_q8: no blocks by the name of %d", plan);
 }

@@ -111,7 +111,7 @@ static int tall_launch(void* C, int c_dtype, const int8_t* X, int64_t pitch, con
 int q8_tall_launch(void* C, int c_dtype, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int gated,
                    GateAct act, int MT, hipStream_t st) {
 #define CASE(T) case T: return tall_launch<T>(C, c_dtype, X, pitch, sx, W, sw, M, N, tiles, chunks, gated, act, st)
-    switch (MT) { CASE(8); CASE(9); CASE(10); CASE(11); CASE(12); CASE(13); CASE(14); CASE(15); CASE(16); }
+    switch (MT) { CASE(8); CASE(10); CASE(12); CASE(14); CASE(16); }
 #undef CASE
     return spy_fail("spy_gemm_q8: %d row tiles", MT);
 }

@@ -356,3 +356,42 @@ def test_a_result_tensor_of_another_kind_is_turned_away():
         ops.add_rms_norm_q8(torch.randn((8, 8), device=dev), torch.randn((8, 8), device=dev).half(), torch.ones(8, device=dev), EPS)
     with pytest.raises(ops.KernelError):
         ops.add_rms_norm_q8(torch.randn((8, 8), device=dev).t(), None, torch.ones(8, device=dev), EPS)
+
+
+#: kinds of blocks of a product (csrc/gemm_q8.hip), and row tiles of each
+PLANS = [101, 102, 103, 104, 201, 202, 203, 204, 206, 404, 406, 408, 8, 10, 12, 14, 16]
+
+
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("T,N,K", [(1, 40, 64), (16, 16, 1), (47, 100, 300), (64, 272, 2300), (130, 70, 1024), (259, 513, 777), (513, 33, 4200)])
+def test_every_kind_of_block(plan, T, N, K, monkeypatch):
+    """Fewer rows, columns and chunks of K than a block has, and more of each; plain and gated, both result types."""
+    from spyinfer_amd.kernels import ops
+    dev = require_gpu()
+    monkeypatch.setattr(ops, "Q8_PLAN", plan)
+    q, sx, p, sw = drawn(T, 2 * N, K, plan + T)
+    sx = sx / 10
+    x = ops.Q8Rows.from_values(q.to(dev), sx.to(dev))
+    want = product64(q, sx, p, sw)
+    w = ops.Q8Weight.from_values(p.to(dev), sw.to(dev))
+    for out in (torch.bfloat16, torch.float32):
+        near(ops.linear_q8(x, w, out), want, (HALF[out] if out != torch.float32 else 0.0) + 3.1 * 2.0 ** -24)
+    narrow = ops.Q8Weight.from_values(p[:N].to(dev), sw[:N].to(dev))
+    near(ops.linear_q8(x, narrow, torch.float32), want[:, :N], 3.1 * 2.0 ** -24)
+    gated = ops.Q8Weight.from_values(p.to(dev), sw.to(dev), gated=True)
+    if plan < 200 and plan > 16:
+        with pytest.raises(ops.KernelError, match="gated"):
+            ops.linear_q8_gated(x, gated)
+        return
+    assert float(want.abs().max()) < 30
+    near(ops.linear_q8_gated(x, gated), activation64(want[:, :N], "silu") * want[:, N:], 2.0 ** -8 + 2.0 ** -13)
+
+
+def test_blocks_that_do_not_exist_are_turned_away(monkeypatch):
+    from spyinfer_amd.kernels import ops
+    dev = require_gpu()
+    x, w = ops.quantize_rows(torch.randn((4, 64), device=dev)), ops.quantize_weight(torch.randn((32, 64), device=dev))
+    for plan in (1, 9, 17, 100, 105, 304, 405, -1):
+        monkeypatch.setattr(ops, "Q8_PLAN", plan)
+        with pytest.raises(ops.KernelError, match="no blocks|row tiles"):
+            ops.linear_q8(x, w)
