@@ -5,79 +5,197 @@
 // The quotient is formed in 64 bits, so that a row's integers are the same however and wherever it is computed: products of two float32 are
 // exact there, and the maximum is one of them.
 // A row of zeros: q 0, scale 0.  A row with a NaN or an infinity: q 0, scale NaN, so that all that is made of it is NaN.
+//
+// Bound by memory: a block takes a row, reads it once, holds it in registers while the maximum (and the sum of squares) goes round, and writes it.
 #include "q8.h"
+#include <type_traits>
 
-__device__ __forceinline__ double block_sum_f64(double v, double* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    const int nw = (blockDim.x + 63) >> 6;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double t = 0.;
-    for (int i = 0; i < nw; ++i) t += red[i];
-    return t;
-}
-// the largest of the values' magnitudes as bits: a NaN is above an infinity, which is above all numbers
-__device__ __forceinline__ unsigned long long block_max_bits(unsigned long long v, unsigned long long* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned long long)__shfl_xor(v, o, 64));
-    const int nw = (blockDim.x + 63) >> 6;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    unsigned long long t = red[0];
-    for (int i = 1; i < nw; ++i) t = max(t, red[i]);
-    return t;
-}
-__device__ __forceinline__ unsigned long long magnitude_bits(double z) { return (unsigned long long)__double_as_longlong(z) & 0x7fffffffffffffffull; }
+// The bits of a value's magnitude: a NaN is above an infinity, which is above all numbers.
+__device__ __forceinline__ unsigned long long magnitude(double z) { return (unsigned long long)__double_as_longlong(z) & 0x7fffffffffffffffull; }
+__device__ __forceinline__ unsigned magnitude(float z) { return __float_as_uint(z) & 0x7fffffffu; }
+__device__ __forceinline__ double value_of(unsigned long long m) { return __longlong_as_double((long long)m); }
+__device__ __forceinline__ double value_of(unsigned m) { return (double)__uint_as_float(m); }
 
-// One block a row.  NORM: x is the residual stream (float32, written with the addend), delta the addend (or null) and weight the norm's; else x are
-// the rows, ldx apart.
+// A row's largest magnitude and its sum, over a block; every thread gets them.
+template <int WAVES, bool SUM, typename BITS>
+__device__ __forceinline__ void row_statistics(BITS& top, double& ss) {
+    __shared__ BITS tops[WAVES];
+    __shared__ double sums[WAVES];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        top = max(top, (BITS)__shfl_xor(top, o, 64));
+        if (SUM) ss += __shfl_xor(ss, o, 64);
+    }
+    if (WAVES == 1) return;
+    if ((threadIdx.x & 63) == 0) { tops[threadIdx.x >> 6] = top; if (SUM) sums[threadIdx.x >> 6] = ss; }
+    __syncthreads();
+    top = tops[0];
+    if (SUM) ss = sums[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) { top = max(top, tops[i]); if (SUM) ss += sums[i]; }
+}
+
+// 127 z / a rounded half to even, z = x or x w.  In 32 bits the quotient is off by up to 3 2^-24 of 127 (the product, 127 / a and theirs), less than 2^-15; adding
+// 1.5 2^23 leaves its nearest integer in the low bits, and only where what that leaves out is half an integer, but for 2^-15, is the quotient itself formed, in 64 bits (one value
+// of 16 000, and ties).  Rows whose largest value is very large or small, for which 127 / a has no 32 bits, go by that altogether (inv NaN).
+template <bool NORM>
+__device__ __forceinline__ int quotient(float x, float w, float inv, double a) {
+    const float u = (NORM ? x * w : x) * inv, t = u + 12582912.f;
+    if (__builtin_expect(!(fabsf(u - (t - 12582912.f)) <= 0.5f - 0x1p-15f), 0)) return (int)rint((NORM ? (double)x * (double)w : (double)x) * 127.0 / a);
+    return (int)__float_as_uint(t);
+}
+
+// What a row's statistics make of it: 127 / a and a (0 and 1 where all integers are 0), and its scale.
+struct RowScale { float inv; double a; float scale; };
+template <bool NORM>
+__device__ __forceinline__ RowScale row_scale(double a, double ss, float eps, int H) {
+    if (!(a < INFINITY)) return {0.f, 1., NAN};
+    if (a == 0.) return {0.f, 1., 0.f};
+    const double scale = a / 127.0;
+    return {a > 0x1p-90 && a < 0x1p120 ? (float)(127.0 / a) : NAN, a, (float)(NORM ? scale / sqrt(ss / (double)H + (double)eps) : scale)};
+}
+
+// VEC values of a row in 16-byte pieces (8: the row is aligned so), or one.
+template <int VEC, typename T>
+__device__ __forceinline__ void load_values(const T* p, float (&v)[VEC]) {
+    if constexpr (VEC == 1) v[0] = to_f32<T>(*p);
+    else if constexpr (sizeof(T) == 4) { Vec4<float>::load(p, v); Vec4<float>::load(p + 4, v + 4); }
+    else {
+        const uint4 t = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(w[e] << 16); v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+    }
+}
+
+// One block a row, held in registers: NP pieces of VEC values a thread.  NORM: x is the residual stream (float32, written with the addend), delta the
+// addend (or null) and weight the norm's; else x are the rows, ldx apart.
+template <typename TX, typename TD, typename TW, bool NORM, int VEC, int THREADS, int NP>
+__global__ __launch_bounds__(THREADS) void rows_q8_kernel(int8_t* __restrict__ q, float* __restrict__ scales, TX* __restrict__ x, int64_t ldx, const TD* __restrict__ delta,
+                                                          const TW* __restrict__ weight, float eps, int H, int64_t pitch) {
+    const size_t row = blockIdx.x;
+    TX* s = x + row * ldx;
+    float v[NP][VEC], w[NP][VEC];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        const int i = (p * THREADS + threadIdx.x) * VEC;
+        if (i < H) {
+            load_values<VEC, TX>(s + i, v[p]);
+            if (NORM) load_values<VEC, TW>(weight + i, w[p]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[p][e] = w[p][e] = 0.f;
+        }
+    }
+    if (NORM && delta) {
+        float d[NP][VEC];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int i = (p * THREADS + threadIdx.x) * VEC;
+            if (i < H) load_values<VEC, TD>(delta + row * H + i, d[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int i = (p * THREADS + threadIdx.x) * VEC;
+            if (i < H) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[p][e] += d[p][e];
+                if constexpr (VEC == 1) s[i] = from_f32<TX>(v[p][0]);
+                else { Vec4<float>::store((float*)s + i, v[p]); Vec4<float>::store((float*)s + i + 4, v[p] + 4); }
+            }
+        }
+    }
+    double ss = 0.;
+    typename std::conditional<NORM, unsigned long long, unsigned>::type top = 0;
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            if constexpr (NORM) {
+                const double z = (double)v[p][e];
+                ss = fma(z, z, ss);
+                top = max(top, magnitude(z * (double)w[p][e]));
+            } else top = max(top, magnitude(v[p][e]));
+        }
+    row_statistics<THREADS / 64, NORM>(top, ss);
+    const RowScale k = row_scale<NORM>(value_of(top), ss, eps, H);
+    if (threadIdx.x == 0) scales[row] = k.scale;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        const int i = (p * THREADS + threadIdx.x) * VEC;
+        if (i >= H) continue;
+        int n[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) n[e] = k.inv == 0.f ? 0 : quotient<NORM>(v[p][e], w[p][e], k.inv, k.a);
+        int8_t* o = q + row * pitch + i;
+        if constexpr (VEC == 1) *o = (int8_t)n[0];
+        else {
+            uint32_t b[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) b[h] = (n[4 * h] & 255) | (n[4 * h + 1] & 255) << 8 | (n[4 * h + 2] & 255) << 16 | (uint32_t)n[4 * h + 3] << 24;
+            *reinterpret_cast<uint2*>(o) = uint2{b[0], b[1]};
+        }
+    }
+}
+
+// The same for rows wider than a block's registers: read twice.
 template <typename TX, typename TD, typename TW, bool NORM>
-__global__ __launch_bounds__(256) void rows_q8_kernel(int8_t* __restrict__ q, float* __restrict__ scales, TX* x, int64_t ldx, const TD* __restrict__ delta,
-                                                      const TW* __restrict__ weight, float eps, int H, int64_t pitch) {
-    __shared__ double red_sum[4];
-    __shared__ unsigned long long red_max[4];
+__global__ __launch_bounds__(1024) void wide_rows_q8_kernel(int8_t* __restrict__ q, float* __restrict__ scales, TX* x, int64_t ldx, const TD* __restrict__ delta,
+                                                            const TW* __restrict__ weight, float eps, int H, int64_t pitch) {
     const size_t row = blockIdx.x;
     TX* s = x + row * ldx;
     double ss = 0.;
-    unsigned long long top = 0;
-    for (int i = threadIdx.x; i < H; i += 256) {
+    typename std::conditional<NORM, unsigned long long, unsigned>::type top = 0;
+    for (int i = threadIdx.x; i < H; i += 1024) {
         float v = to_f32<TX>(s[i]);
-        double z = v;
-        if (NORM) {
-            if (delta) { v += to_f32<TD>(delta[row * H + i]); s[i] = from_f32<TX>(v); }
+        if (NORM && delta) { v += to_f32<TD>(delta[row * H + i]); s[i] = from_f32<TX>(v); }
+        if constexpr (NORM) {
             ss = fma((double)v, (double)v, ss);
-            z = (double)v * (double)to_f32<TW>(weight[i]);
-        }
-        top = max(top, magnitude_bits(z));
+            top = max(top, magnitude((double)v * (double)to_f32<TW>(weight[i])));
+        } else top = max(top, magnitude(v));
     }
-    top = block_max_bits(top, red_max);
-    const double a = __longlong_as_double((long long)top);
-    double scale = a / 127.0;
-    if (NORM) scale /= sqrt(block_sum_f64(ss, red_sum) / (double)H + (double)eps);
-    const bool some = a > 0. && a < INFINITY;
-    if (threadIdx.x == 0) scales[row] = a < INFINITY ? (a > 0. ? (float)scale : 0.f) : NAN;
-    for (int i = threadIdx.x; i < H; i += 256) {
-        double z = to_f32<TX>(s[i]);              // (this thread wrote it above)
-        if (NORM) z *= (double)to_f32<TW>(weight[i]);
-        q[row * pitch + i] = some ? (int8_t)(int)rint(z * 127.0 / a) : (int8_t)0;
-    }
+    row_statistics<16, NORM>(top, ss);
+    const RowScale k = row_scale<NORM>(value_of(top), ss, eps, H);
+    if (threadIdx.x == 0) scales[row] = k.scale;
+    for (int i = threadIdx.x; i < H; i += 1024)                // (what a thread reads of the stream, it wrote itself)
+        q[row * pitch + i] = k.inv == 0.f ? (int8_t)0 : (int8_t)quotient<NORM>(to_f32<TX>(s[i]), NORM ? to_f32<TW>(weight[i]) : 1.f, k.inv, k.a);
+}
+
+template <typename TX, typename TD, typename TW, bool NORM>
+static void rows_launch(int8_t* q, float* scales, TX* x, int64_t ldx, const TD* delta, const TW* weight, float eps, int T, int H, int64_t pitch, hipStream_t st) {
+#define ROWS(VEC, THREADS, NP) rows_q8_kernel<TX, TD, TW, NORM, VEC, THREADS, NP><<<T, THREADS, 0, st>>>(q, scales, x, ldx, delta, weight, eps, H, pitch)
+    const bool vec = H % 8 == 0 && ldx % (16 / sizeof(TX)) == 0 && (((uintptr_t)x | (uintptr_t)delta | (uintptr_t)weight) % 16) == 0;
+    const bool few = T <= 512;               // (blocks for all compute units are there anyway, or a thread has as little to do as possible)
+    if (vec && H <= 512) ROWS(8, 64, 1);
+    else if (vec && H <= 2048) ROWS(8, 256, 1);
+    else if (vec && H <= 4096) { if (few) ROWS(8, 512, 1); else ROWS(8, 256, 2); }
+    else if (vec && H <= 8192 && few) ROWS(8, 1024, 1);
+    else if (vec && H <= 6144) ROWS(8, 256, 3);
+    else if (vec && H <= 8192) ROWS(8, 512, 2);
+    else if (vec && H <= 16384 && few) ROWS(8, 1024, 2);
+    else if (vec && H <= 12288) ROWS(8, 512, 3);
+    else if (vec && H <= 16384) ROWS(8, 512, 4);
+    else if (vec && H <= 24576) ROWS(8, 1024, 3);
+    else if (vec && H <= 32768) ROWS(8, 1024, 4);
+    else if (H <= 1024) ROWS(1, 256, 4);
+    else if (H <= 4096) ROWS(1, 1024, 4);
+    else if (H <= 16384) ROWS(1, 1024, 16);
+    else wide_rows_q8_kernel<TX, TD, TW, NORM><<<T, 1024, 0, st>>>(q, scales, x, ldx, delta, weight, eps, H, pitch);
+#undef ROWS
 }
 
 extern "C" int spy_add_rmsnorm_q8(void* q, float* scales, float* stream, const void* delta, int delta_dtype, const void* weight, int weight_dtype, float eps,
                                   int T, int H, int64_t pitch, hipStream_t st) {
-    SPY_REQUIRE(T > 0 && H > 0 && pitch >= H, "spy_add_rmsnorm_q8: bad sizes %d x %d", T, H);
-    SPY_DISPATCH(delta_dtype, TD, SPY_DISPATCH(weight_dtype, TW, rows_q8_kernel<float, TD, TW, true><<<T, 256, 0, st>>>(
-        (int8_t*)q, scales, stream, (int64_t)H, (const TD*)delta, (const TW*)weight, eps, H, pitch)));
+    SPY_REQUIRE(T > 0 && H > 0 && pitch >= H && pitch % 16 == 0 && (uintptr_t)q % 16 == 0, "spy_add_rmsnorm_q8: bad sizes %d x %d", T, H);
+    SPY_DISPATCH(delta_dtype, TD, SPY_DISPATCH(weight_dtype, TW, rows_launch<float, TD, TW, true>(
+        (int8_t*)q, scales, stream, (int64_t)H, (const TD*)delta, (const TW*)weight, eps, T, H, pitch, st)));
     SPY_CHECK_LAUNCH("spy_add_rmsnorm_q8");
     return 0;
 }
 
 extern "C" int spy_quantize_rows(void* q, float* scales, const void* x, int x_dtype, int64_t ldx, int T, int H, int64_t pitch, hipStream_t st) {
-    SPY_REQUIRE(T > 0 && H > 0 && pitch >= H && ldx >= H, "spy_quantize_rows: bad sizes %d x %d", T, H);
-    SPY_DISPATCH(x_dtype, TX, rows_q8_kernel<TX, float, float, false><<<T, 256, 0, st>>>((int8_t*)q, scales, (TX*)x, ldx, nullptr, nullptr, 0.f, H, pitch));
+    SPY_REQUIRE(T > 0 && H > 0 && pitch >= H && pitch % 16 == 0 && (uintptr_t)q % 16 == 0 && ldx >= H, "spy_quantize_rows: bad sizes %d x %d", T, H);
+    SPY_DISPATCH(x_dtype, TX, rows_launch<TX, float, float, false>((int8_t*)q, scales, (TX*)x, ldx, nullptr, nullptr, 0.f, T, H, pitch, st));
     SPY_CHECK_LAUNCH("spy_quantize_rows");
     return 0;
 }

@@ -120,14 +120,6 @@ class _Hip:
         return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on_device_of(t: torch.Tensor):
-    """Launches inside go to the current stream of the device that ``t`` lies on."""
-    return _HERE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
-
-
 def hip() -> _Hip:
     global _hip
     if _hip is None:
@@ -2739,17 +2731,20 @@ Q8_MAX_WIDTH = 511 * 256
 #: 0: the kernels' own rule; else the blocks of the next products by name (csrc/gemm_q8.hip), for tests of every kind of block
 Q8_PLAN = 0
 
-
-def _q8_pitch(width: int) -> int:
-    return (width + 15) & ~15
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
 class Q8Rows:
-    """Rows in 8-bit integers: row t stands for ``values[t, :width]`` times ``scales[t]``.  ``values`` int8 [T, pitch], pitch the
+    """Rows in 8-bit integers: row t stands for ``values[t, :width]`` times ``scales[t]``.  ``values`` int8 [T, pitch], dense, pitch the
     width rounded up to 16 (what lies behind a row's end is anything); ``scales`` float32 [T]."""
     __slots__ = ("values", "scales", "width")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, width: int):
+        _check(values.dtype == torch.int8 and values.dim() == 2 and width > 0 and values.shape[1] == (width + 15) & -16 and values.is_contiguous()
+               and values.data_ptr() % 16 == 0, "Q8Rows: dense int8 values [T, width rounded up to 16] expected")
+        _check(tuple(scales.shape) == (values.shape[0],) and scales.dtype == torch.float32 and scales.is_contiguous() and scales.device == values.device,
+               "Q8Rows: a float32 scale for each row expected")
         self.values, self.scales, self.width = values, scales, width
 
     shape = property(lambda self: (self.values.shape[0], self.width))
@@ -2759,18 +2754,23 @@ class Q8Rows:
     def from_values(values: torch.Tensor, scales: torch.Tensor) -> "Q8Rows":
         """``values`` int8 [T, K] with a scale for each row, float32 [T]."""
         _check(values.dim() == 2 and values.dtype == torch.int8 and values.shape[1] > 0, "Q8Rows: int8 values [T, K] expected")
-        _check(tuple(scales.shape) == (values.shape[0],) and scales.dtype == torch.float32, "Q8Rows: a float32 scale for each row expected")
         T, K = values.shape
         if K % 16 or not values.is_contiguous() or values.data_ptr() % 16:
-            kept = torch.zeros((T, _q8_pitch(K)), dtype=torch.int8, device=values.device)
+            kept = torch.zeros((T, (K + 15) & -16), dtype=torch.int8, device=values.device)
             kept[:, :K] = values
             values = kept
-        _dev(values, scales)
         return Q8Rows(values, scales, K)
 
     def to_rows(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values that the rows stand for, [T, K], each rounded once to ``dtype``."""
         return (self.values[:, :self.width].double() * self.scales[:, None]).to(dtype)
+
+
+def _new_q8_rows(like: torch.Tensor, T: int, width: int) -> Q8Rows:
+    """Rows to be written, on the device of ``like`` (made without the constructor's checks: a step has hundreds)."""
+    rows = Q8Rows.__new__(Q8Rows)
+    rows.values, rows.scales, rows.width = like.new_empty((T, (width + 15) & -16), dtype=torch.int8), like.new_empty((T,), dtype=torch.float32), width
+    return rows
 
 
 class Q8Weight:
@@ -2785,7 +2785,15 @@ class Q8Weight:
     dtype = torch.int8
 
     def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, shape, gated: bool):
-        self.tiles, self.scales, self.shape, self.gated = tiles, scales, torch.Size(shape), gated
+        N, K = shape
+        halves = 2 if gated else 1
+        _check(N > 0 and K > 0 and N % halves == 0, "Q8Weight: %d rows are no gate and up rows", N)
+        count = halves * (-(-(N // halves) // 16))
+        _check(tiles.dtype == torch.int8 and tuple(tiles.shape) == (-(-K // 256), count, 4, 4, 16, 16) and tiles.is_contiguous() and tiles.data_ptr() % 16 == 0,
+               "Q8Weight: tiles of a matrix of %d x %d expected", N, K)
+        _check(tuple(scales.shape) == (16 * count,) and scales.dtype == torch.float32 and scales.is_contiguous() and scales.device == tiles.device,
+               "Q8Weight: a float32 scale for each row of the tiles expected")
+        self.tiles, self.scales, self.shape, self.gated = tiles, scales, torch.Size((N, K)), bool(gated)
 
     def dim(self) -> int:
         return 2
@@ -2801,14 +2809,15 @@ class Q8Weight:
         _check(N % halves == 0, "Q8Weight: %d rows are no gate and up rows", N)
         _check(K <= Q8_MAX_WIDTH, "Q8Weight: a width of %d, the sums hold %d", K, Q8_MAX_WIDTH)
         _check(bool(torch.isfinite(scales).all()), "Q8Weight: a row's scale is no finite number")
-        rows, width = -(-(N // halves) // 16) * 16, -(-K // 256) * 256
+        half, rows, width = N // halves, -(-(N // halves) // 16) * 16, -(-K // 256) * 256
         _check(halves * rows * width < 1 << 31, "Q8Weight: a matrix of %d x %d is too large", N, K)
-        full = values.new_zeros((halves, rows, width))
-        full[:, :N // halves, :K] = values.view(halves, N // halves, K)
-        tiles = full.view(halves * rows // 16, 16, width // 256, 4, 4, 16).permute(2, 0, 3, 4, 1, 5).contiguous()
-        kept = scales.new_zeros((halves, rows))
-        kept[:, :N // halves] = scales.view(halves, N // halves)
-        return Q8Weight(tiles, kept.view(-1), (N, K), bool(gated))
+        if (rows, width) != (half, K):
+            full, kept = values.new_zeros((halves, rows, width)), scales.new_zeros((halves, rows))
+            full[:, :half, :K] = values.reshape(halves, half, K)
+            kept[:, :half] = scales.view(halves, half)
+            values, scales = full, kept
+        tiles = values.reshape(halves * rows // 16, 16, width // 256, 4, 4, 16).permute(2, 0, 3, 4, 1, 5).contiguous()
+        return Q8Weight(tiles, scales.reshape(-1).contiguous(), (N, K), gated)
 
     def to_rows(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The matrix that the integers stand for, [N, K], each value rounded once to ``dtype``."""
@@ -2823,24 +2832,28 @@ def quantize_weight(w: torch.Tensor, gated: bool = False) -> Q8Weight:
     """``w [N, K]`` (float32 or bfloat16) as a ``Q8Weight``: every row's integers are 127 w / max |w| rounded half to even, its
     scale max |w| / 127."""
     rows = quantize_rows(w)
-    return Q8Weight.from_values(rows.values[:, :rows.width].contiguous(), rows.scales, gated)
+    return Q8Weight.from_values(rows.values[:, :rows.width], rows.scales, gated)
 
 
 def quantize_rows(x: torch.Tensor) -> Q8Rows:
     """Rows ``x [T, K]`` (float32 or bfloat16; they may be a view into the rows of a wider tensor) in 8-bit integers: 127 x / a rounded half to
     even, a = max |x| of the row, and the scale a / 127.  A row of zeros has zeros and the scale 0; one with a NaN or an infinity zeros and the
     scale NaN, so that all that is made of it is NaN."""
-    _check(x.is_cuda and x.dim() == 2 and x.dtype in _CODES and x.shape[1] > 0, "quantize_rows: float32 or bfloat16 rows [T, K] on the GPU expected")
-    T, K = x.shape
-    _check(T <= 1 or (x.stride(1) == 1 or K == 1) and x.stride(0) >= K, "quantize_rows: dense rows, or rows of a wider tensor, expected")
-    _check(T > 1 or K == 1 or x.stride(1) == 1, "quantize_rows: dense rows, or rows of a wider tensor, expected")
-    with _on_device_of(x):
-        values = torch.empty((T, _q8_pitch(K)), dtype=torch.int8, device=x.device)
-        scales = torch.empty((T,), dtype=torch.float32, device=x.device)
-        if T:
-            hip().call("spy_quantize_rows", values.data_ptr(), scales.data_ptr(), x.data_ptr(), _CODES[x.dtype], max(x.stride(0), K) if T > 1 else K, T, K,
-                       values.shape[1], _Hip.stream())
-    return Q8Rows(values, scales, K)
+    code = _CODES.get(x.dtype)
+    if code is None or x.dim() != 2 or not x.is_cuda:
+        raise KernelError("quantize_rows: float32 or bfloat16 rows [T, K] on the GPU expected")
+    (T, K), (ld, step) = x.shape, x.stride()
+    if K == 0 or (step != 1 and K > 1) or (ld < K and T > 1):
+        raise KernelError("quantize_rows: dense rows, or rows of a wider tensor, expected")
+    device = x.get_device()
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return quantize_rows(x)
+    rows = _new_q8_rows(x, T, K)
+    if T:
+        hip().call("spy_quantize_rows", rows.values.data_ptr(), rows.scales.data_ptr(), x.data_ptr(), code, ld if T > 1 else K, T, K, (K + 15) & -16,
+                   _raw_stream(device))
+    return rows
 
 
 def _q8_rows(x) -> Q8Rows:
@@ -2852,48 +2865,68 @@ def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
     each row, as ``quantize_rows`` has them (of the norm's result in full, not of one rounded to bfloat16).  ``delta``: [T, H] float32 or
     bfloat16."""
     _dev(resid, delta, weight)
-    _check(resid.dtype == torch.float32 and resid.dim() == 2 and resid.shape[1] > 0, "add_rms_norm_q8: the residual stream must be float32 [T, H]")
+    if resid.dtype != torch.float32 or resid.dim() != 2 or resid.shape[1] == 0:
+        raise KernelError("add_rms_norm_q8: the residual stream must be float32 [T, H]")
     T, H = resid.shape
-    _check(weight.shape == (H,) and weight.dtype in _CODES, "add_rms_norm_q8: weight must be [H], float32 or bfloat16")
-    _check(delta is None or (delta.shape == resid.shape and delta.dtype in _CODES), "add_rms_norm_q8: delta must be [T, H], float32 or bfloat16")
-    with _on_device_of(resid):
-        values = torch.empty((T, _q8_pitch(H)), dtype=torch.int8, device=resid.device)
-        scales = torch.empty((T,), dtype=torch.float32, device=resid.device)
-        if T:
-            hip().call("spy_add_rmsnorm_q8", values.data_ptr(), scales.data_ptr(), resid.data_ptr(), 0 if delta is None else delta.data_ptr(),
-                       0 if delta is None else _CODES[delta.dtype], weight.data_ptr(), _CODES[weight.dtype], eps, T, H, values.shape[1], _Hip.stream())
-    return Q8Rows(values, scales, H)
+    weight_code, delta_code = _CODES.get(weight.dtype), F32 if delta is None else _CODES.get(delta.dtype)
+    if weight_code is None or weight.shape != (H,):
+        raise KernelError("add_rms_norm_q8: weight must be [H], float32 or bfloat16")
+    if delta_code is None or (delta is not None and delta.shape != resid.shape):
+        raise KernelError("add_rms_norm_q8: delta must be [T, H], float32 or bfloat16")
+    device = resid.get_device()
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return add_rms_norm_q8(resid, delta, weight, eps)
+    rows = _new_q8_rows(resid, T, H)
+    if T:
+        hip().call("spy_add_rmsnorm_q8", rows.values.data_ptr(), rows.scales.data_ptr(), resid.data_ptr(), None if delta is None else delta.data_ptr(), delta_code,
+                   weight.data_ptr(), weight_code, eps, T, H, (H + 15) & -16, _raw_stream(device))
+    return rows
 
 
-def _gemm_q8(x: Q8Rows, w: Q8Weight, out: torch.Tensor, columns: int, act: int) -> torch.Tensor:
-    if out.shape[0]:
-        with _on_device_of(out):
-            hip().call("spy_gemm_q8", out.data_ptr(), _CODES[out.dtype], x.values.data_ptr(), x.values.shape[1], x.scales.data_ptr(), w.tiles.data_ptr(),
-                       w.scales.data_ptr(), out.shape[0], columns, w.tiles.shape[1], w.tiles.shape[0], 1 if w.gated else 0, act, Q8_PLAN, _Hip.stream())
+def _gemm_q8(name: str, x: Q8Rows, w: Q8Weight, out_dtype: torch.dtype, out: Optional[torch.Tensor], columns: int, act: int) -> torch.Tensor:
+    values, tiles = x.values, w.tiles
+    if x.width != w.shape[1]:
+        raise KernelError("%s: rows of %d and a matrix of %d x %d" % (name, x.width, w.shape[0], w.shape[1]))
+    device = values.get_device()
+    if not (values.is_cuda and tiles.is_cuda):
+        raise KernelError("%s: an operand lies on the CPU; the kernels run on the GPU only" % name)
+    if tiles.get_device() != device:
+        raise KernelError("%s: operands lie on different devices" % name)
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return _gemm_q8(name, x, w, out_dtype, out, columns, act)
+    T, pitch = values.shape
+    out = values.new_empty((T, columns), dtype=out_dtype) if out is None else _result(out, T, columns, out_dtype, values.device)
+    if T:
+        hip().call("spy_gemm_q8", out.data_ptr(), _CODES[out_dtype], values.data_ptr(), pitch, x.scales.data_ptr(), tiles.data_ptr(), w.scales.data_ptr(), T, columns,
+                   tiles.shape[1], tiles.shape[0], 1 if w.gated else 0, act, Q8_PLAN, _raw_stream(device))
     return out
 
 
 def linear_q8(x: Q8Rows, w: Q8Weight, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = x . w^T of rows and a matrix in 8-bit integers: the sums of products are 32-bit integers, exact; a sum times its row's and
     its column's scale is rounded once, to ``out_dtype`` (bfloat16 or float32).  ``out``: the result is written there."""
-    _check(isinstance(x, Q8Rows) and isinstance(w, Q8Weight), "linear_q8: Q8Rows and a Q8Weight expected")
-    _check(not w.gated, "linear_q8: a matrix of gate and up rows goes to linear_q8_gated")
-    _check(x.width == w.shape[1], "linear_q8: rows of %d and a matrix of %d x %d", x.width, w.shape[0], w.shape[1])
-    _check(out_dtype in _CODES, "linear_q8: output dtype must be float32 or bfloat16")
-    _dev(x.values, x.scales, w.tiles, w.scales)
-    return _gemm_q8(x, w, _result(out, x.values.shape[0], w.shape[0], out_dtype, x.values.device), w.shape[0], 0)
+    if not (isinstance(x, Q8Rows) and isinstance(w, Q8Weight)):
+        raise KernelError("linear_q8: Q8Rows and a Q8Weight expected")
+    if w.gated:
+        raise KernelError("linear_q8: a matrix of gate and up rows goes to linear_q8_gated")
+    if out_dtype not in _CODES:
+        raise KernelError("linear_q8: output dtype must be float32 or bfloat16")
+    return _gemm_q8("linear_q8", x, w, out_dtype, out, w.shape[0], 0)
 
 
 def linear_q8_gated(x: Q8Rows, w: Q8Weight, activation: str = "silu") -> torch.Tensor:
     """act(x . Wgate^T) * (x . Wup^T) -> bfloat16 [M, N / 2] for a matrix of [gate | up] rows, the two values formed as in
     ``linear_q8`` and rounded once, after the activation.  ``activation``: one of GATED_ACTIVATIONS."""
-    _check(isinstance(x, Q8Rows) and isinstance(w, Q8Weight), "linear_q8_gated: Q8Rows and a Q8Weight expected")
-    _check(w.gated, "linear_q8_gated: a matrix of [gate | up] rows expected")
-    _check(x.width == w.shape[1], "linear_q8_gated: rows of %d and a matrix of %d x %d", x.width, w.shape[0], w.shape[1])
-    _check(activation in GATED_ACTIVATIONS, "linear_q8_gated: activation %r is not implemented", activation)
-    _dev(x.values, x.scales, w.tiles, w.scales)
-    out = torch.empty((x.values.shape[0], w.shape[0] // 2), dtype=torch.bfloat16, device=x.values.device)
-    return _gemm_q8(x, w, out, w.shape[0] // 2, GATED_ACTIVATIONS[activation])
+    if not (isinstance(x, Q8Rows) and isinstance(w, Q8Weight)):
+        raise KernelError("linear_q8_gated: Q8Rows and a Q8Weight expected")
+    if not w.gated:
+        raise KernelError("linear_q8_gated: a matrix of [gate | up] rows expected")
+    act = GATED_ACTIVATIONS.get(activation)
+    if act is None:
+        raise KernelError("linear_q8_gated: activation %r is not implemented" % (activation,))
+    return _gemm_q8("linear_q8_gated", x, w, torch.bfloat16, None, w.shape[0] // 2, act)
 
 
 # --------------------------------------------------------------------------

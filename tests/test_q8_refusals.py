@@ -29,6 +29,13 @@ def weight(n=32, k=32, gated=False):
     (lambda: ops.linear_q8_gated(rows(), weight(gated=True), "relu"), "relu"),
     (lambda: ops.linear_q8_gated(rows(), weight(gated=True)), "GPU only"),
     (lambda: ops.quantize_weight(torch.zeros(4, 8)), "on the GPU"),
+    (lambda: Q8Rows(torch.zeros((2, 33), dtype=torch.int8), torch.ones(2), 33), "rounded up to 16"),
+    (lambda: Q8Rows(torch.zeros((2, 48), dtype=torch.int8), torch.ones(2), 32), "rounded up to 16"),
+    (lambda: Q8Rows(torch.zeros((48, 2), dtype=torch.int8).t(), torch.ones(2), 48), "dense"),
+    (lambda: Q8Rows(torch.zeros((2, 48), dtype=torch.int8), torch.ones(4)[::2], 48), "scale"),
+    (lambda: Q8Weight(torch.zeros((1, 2, 4, 4, 16, 16), dtype=torch.int8), torch.ones(16), (32, 256), False), "scale"),
+    (lambda: Q8Weight(torch.zeros((1, 2, 4, 4, 16, 16), dtype=torch.int8), torch.ones(32), (33, 256), False), "tiles"),
+    (lambda: Q8Weight(torch.zeros((1, 2, 4, 4, 16, 16), dtype=torch.int8), torch.ones(32), (31, 256), True), "gate and up"),
     (lambda: Q8Rows.from_values(torch.zeros(2, 8), torch.ones(2)), "int8"),
     (lambda: Q8Rows.from_values(torch.zeros((2, 8), dtype=torch.int8), torch.ones(3)), "scale"),
     (lambda: Q8Weight.from_values(torch.zeros(2, 8), torch.ones(2)), "int8"),
