@@ -15,6 +15,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import math
 import threading
 from typing import Optional
 
@@ -2808,7 +2809,7 @@ class Q8Weight:
         halves = 2 if gated else 1
         _check(N % halves == 0, "Q8Weight: %d rows are no gate and up rows", N)
         _check(K <= Q8_MAX_WIDTH, "Q8Weight: a width of %d, the sums hold %d", K, Q8_MAX_WIDTH)
-        _check(bool(torch.isfinite(scales).all()), "Q8Weight: a row's scale is no finite number")
+        _check(math.isfinite(scales.abs().amax().item()), "Q8Weight: a row's scale is no finite number")       # (a NaN is the largest of all)
         half, rows, width = N // halves, -(-(N // halves) // 16) * 16, -(-K // 256) * 256
         _check(halves * rows * width < 1 << 31, "Q8Weight: a matrix of %d x %d is too large", N, K)
         if (rows, width) != (half, K):
@@ -2816,7 +2817,8 @@ class Q8Weight:
             full[:, :half, :K] = values.reshape(halves, half, K)
             kept[:, :half] = scales.view(halves, half)
             values, scales = full, kept
-        tiles = values.reshape(halves * rows // 16, 16, width // 256, 4, 4, 16).permute(2, 0, 3, 4, 1, 5).contiguous()
+        words = values.contiguous().view(-1).view(torch.int64) if values.data_ptr() % 8 == 0 else values.clone().view(-1).view(torch.int64)
+        tiles = words.view(halves * rows // 16, 16, width // 256, 4, 4, 2).permute(2, 0, 3, 4, 1, 5).contiguous().view(torch.int8)
         return Q8Weight(tiles, scales.reshape(-1).contiguous(), (N, K), gated)
 
     def to_rows(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:

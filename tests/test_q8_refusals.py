@@ -69,3 +69,13 @@ def test_rows_of_any_width_are_kept_in_pieces_of_16():
     r = Q8Rows(torch.zeros((2, 48), dtype=torch.int8), torch.tensor([2.0, 0.5]), 33)
     r.values[:, :33] = q
     assert torch.equal(r.to_rows(), q.float() * r.scales[:, None]) and r.shape == (2, 33)
+
+
+def test_a_matrix_from_any_place_in_memory():
+    """Values that begin at any byte, rows of a wider tensor, and scales whose sum is no float32."""
+    g = torch.Generator().manual_seed(1)
+    flat = torch.randint(-128, 128, (3 + 32 * 256,), generator=g, dtype=torch.int8)
+    p, s = flat[3:].view(32, 256), torch.full((32,), 3e38)
+    assert torch.equal(Q8Weight.from_values(p, s).to_rows(torch.float64), p.double() * s[:, None].double())
+    wide = torch.randint(-128, 128, (32, 600), generator=g, dtype=torch.int8)
+    assert torch.equal(Q8Weight.from_values(wide[:, 5:261], s).to_rows(torch.float64), wide[:, 5:261].double() * s[:, None].double())
