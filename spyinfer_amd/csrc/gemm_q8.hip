@@ -170,17 +170,17 @@ static int split_launch(const Q8Args& a) {
 }
 
 // Which blocks: those with the least estimated time, us, of c[0] + c[1] r k + c[2] r + c[3] b k + c[4] x, b the blocks over 256 compute units, r that rounded up,
-// k the chunks of K; x: chunks of K that row tiles bring over the units, x k (tall blocks: b).  Fitted to 2720 products of 1 to 4096 rows, 256 to 34816 columns and K of 512 to 17408,
-// plain and gated, each with the matrices from memory, in every kind of block (4 to 13 % rms); what it takes is 1.3 % slower on average than the
-// fastest of all kinds, 7.5 % at the 95th percentile.  NT 100 + MT, or, tall, the row tiles alone.
+// k the chunks of K; x: chunks of K that row tiles bring over the units, x k (tall blocks: b).  Fitted to 4500 products of 1 to 8192 rows, 16 to 34816 columns and K of 512 to 17408,
+// plain and gated, each with the matrices from memory, in every kind of block (6 to 19 % rms, the short products' least exactly); what it takes is 1.1 % slower on average than the
+// fastest kind, 6.6 % at the 95th percentile.  NT 100 + MT, or, tall, the row tiles alone.
 struct Q8Cost { int plan; float c[5]; };
 static const Q8Cost q8_costs[] = {
-    {101, {2.48f, 0.0793f, 0.627f, 0.f, 0.0674f}}, {102, {2.43f, 0.117f, 0.859f, 0.f, 0.0457f}}, {103, {2.37f, 0.154f, 1.19f, 0.f, 0.0351f}},
-    {104, {1.87f, 0.169f, 2.04f, 0.0456f, 0.00598f}}, {201, {2.44f, 0.141f, 0.504f, 0.149f, 0.f}}, {202, {2.44f, 0.168f, 0.741f, 0.0611f, 0.0554f}},
-    {203, {2.54f, 0.203f, 0.927f, 0.0379f, 0.0502f}}, {204, {2.8f, 0.218f, 1.06f, 0.0824f, 0.f}}, {206, {1.64f, 0.248f, 2.78f, 0.f, 0.0279f}},
-    {404, {3.43f, 0.277f, 1.45f, 0.192f, 0.f}}, {406, {1.55f, 0.363f, 4.58f, 0.f, 0.0354f}}, {408, {1.84f, 0.464f, 5.66f, 0.f, 0.0248f}},
-    {8, {2.26f, 1.08f, 3.97f, 0.584f, 3.25f}}, {10, {1.96f, 1.28f, 5.09f, 0.512f, 4.28f}}, {12, {1.61f, 1.44f, 6.05f, 0.579f, 4.88f}},
-    {14, {0.833f, 1.65f, 7.43f, 0.625f, 5.73f}}, {16, {0.011f, 1.88f, 8.71f, 0.647f, 6.44f}},
+    {101, {2.69f, 0.0642f, 0.357f, 0.0601f, 0.f}}, {102, {2.63f, 0.0924f, 0.604f, 0.0807f, 0.000247f}}, {103, {2.52f, 0.134f, 0.935f, 0.052f, 0.0149f}},
+    {104, {1.6f, 0.164f, 2.1f, 0.0426f, 0.0122f}}, {201, {2.87f, 0.112f, 0.106f, 0.0753f, 0.f}}, {202, {2.98f, 0.126f, 0.213f, 0.136f, 0.f}},
+    {203, {2.91f, 0.176f, 0.566f, 0.127f, 0.f}}, {204, {2.77f, 0.208f, 0.97f, 0.103f, 0.f}}, {206, {1.95f, 0.254f, 2.51f, 0.f, 0.0292f}},
+    {404, {3.58f, 0.273f, 1.29f, 0.2f, 0.f}}, {406, {1.79f, 0.371f, 4.28f, 0.f, 0.0375f}}, {408, {2.46f, 0.459f, 5.05f, 0.f, 0.0294f}},
+    {8, {2.09f, 0.999f, 4.72f, 0.637f, 2.45f}}, {10, {1.8f, 1.23f, 5.85f, 0.548f, 3.4f}}, {12, {1.49f, 1.4f, 6.95f, 0.631f, 3.75f}},
+    {14, {0.754f, 1.58f, 8.58f, 0.723f, 4.18f}}, {16, {0.0796f, 1.83f, 9.34f, 0.735f, 5.32f}},
 };
 
 static int q8_plan(int M, int tiles, int chunks, int gated) {
@@ -190,8 +190,8 @@ static int q8_plan(int M, int tiles, int chunks, int gated) {
     for (const Q8Cost& p : q8_costs) {
         const bool tall = p.plan < 100;
         const int MT = tall ? p.plan : p.plan % 100, NO = tall ? (gated ? 8 : 16) : p.plan / 100 / (gated ? 2 : 1);
-        // up to three row tiles: as many as there are; more: not many more than there are (four from 33 rows on, six from 81, eight from 113, tall from 65)
-        if (NO < 1 || (tall ? M <= 64 : MT < 4 ? row_tiles != MT : MT == 4 ? row_tiles < 3 : row_tiles < MT)) continue;
+        // not many more row tiles than there are (four from 33 rows on, six from 81, eight from 113, tall from 65)
+        if (NO < 1 || (tall ? M <= 64 : MT == 4 ? row_tiles < 3 : row_tiles < MT)) continue;
         const int cols = (col_tiles + NO - 1) / NO;
         const float blocks = (float)((row_tiles + MT - 1) / MT) * (float)cols / 256.f, rounds = ceilf(blocks), k = (float)chunks;
         const float us = p.c[0] + p.c[1] * rounds * k + p.c[2] * rounds + p.c[3] * blocks * k + p.c[4] * (tall ? blocks : (float)row_tiles * cols / 256.f * k);

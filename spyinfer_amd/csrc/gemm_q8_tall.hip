@@ -20,7 +20,7 @@ __device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t
     constexpr int CT = MT / 4, VEC = 16 / sizeof(TC), PIECES = (EPI == Q8_GATED ? 32 : 64) / VEC, ROWS = 64 / PIECES;
     int* mine = reinterpret_cast<int*>(stage) + wave * CT * 16 * 64;
     const int r = lane & 15, g = lane >> 4, q = (lane % PIECES) * (VEC / 4), column = at + q * 4;
-    const bool whole = ld % VEC == 0 && (uintptr_t)out % 16 == 0 && column + VEC <= columns;
+    const bool whole = ld % VEC == 0 && (uintptr_t)out % 16 == 0;              // (a piece then exists whole or not at all)
     float fw[VEC], fu[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
@@ -35,24 +35,36 @@ __device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t
             for (int j = 0; j < 4; ++j) *reinterpret_cast<q8_i32x4_t*>(mine + ((i - i0) * 16 + r) * 64 + ((j * 4 + g) ^ r) * 4) = acc[j][i];
         __builtin_amdgcn_sched_barrier(0);
         const int here = min(16 * min(CT, MT - i0), rows - i0 * 16);
-#pragma unroll 1
-        for (int row = lane / PIECES; row < here; row += ROWS) {
-            const int* from = mine + row * 64;
-            const float fx = sx[i0 * 16 + row];
-            float v[VEC];
+        if (whole || sizeof(TC) == 2) {
+#pragma unroll 2
+            for (int row = lane / PIECES; row < here; row += ROWS) {
+                const int* from = mine + row * 64;
+                const float fx = sx[i0 * 16 + row];
+                float v[VEC];
 #pragma unroll
-            for (int k = 0; k < VEC / 4; ++k) {
-                const q8_i32x4_t a = *reinterpret_cast<const q8_i32x4_t*>(from + ((q + k) ^ (row & 15)) * 4);
-                const q8_i32x4_t b = *reinterpret_cast<const q8_i32x4_t*>(from + ((q + k + (EPI == Q8_GATED ? 8 : 0)) ^ (row & 15)) * 4);
+                for (int k = 0; k < VEC / 4; ++k) {
+                    const q8_i32x4_t a = *reinterpret_cast<const q8_i32x4_t*>(from + ((q + k) ^ (row & 15)) * 4);
+                    const q8_i32x4_t b = *reinterpret_cast<const q8_i32x4_t*>(from + ((q + k + (EPI == Q8_GATED ? 8 : 0)) ^ (row & 15)) * 4);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[k * 4 + e] = q8_value<EPI>(act, a[e], b[e], fx, fw[k * 4 + e], fu[k * 4 + e]);
+                    for (int e = 0; e < 4; ++e) v[k * 4 + e] = q8_value<EPI>(act, a[e], b[e], fx, fw[k * 4 + e], fu[k * 4 + e]);
+                }
+                TC* o = out + (int64_t)(i0 * 16 + row) * ld + column;
+                if (whole) { if (column < columns) q8_store_piece(o, v); }
+                else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (column + e < columns) o[e] = from_f32<TC>(v[e]);
+                }
             }
-            TC* o = out + (int64_t)(i0 * 16 + row) * ld + column;
-            if (whole) q8_store_piece(o, v);
-            else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    if (column + e < columns) o[e] = from_f32<TC>(v[e]);
+        } else {
+            // float32 rows that begin anywhere: a lane has a column (of bfloat16 that is slower than single values of a piece: 2228 rows, 4096 -> 705 28.3 / 31.8 us)
+            const int c = lane;
+            const bool is = at + c < columns;
+            const float cw = is ? sw[at + c] : 0.f;
+#pragma unroll 8
+            for (int row = 0; row < here; ++row) {
+                const int a = mine[row * 64 + ((c / 4) ^ (row & 15)) * 4 + c % 4];
+                if (is) out[(int64_t)(i0 * 16 + row) * ld + at + c] = from_f32<TC>(q8_value<Q8_STORE>(act, a, a, sx[i0 * 16 + row], cw, 0.f));
             }
         }
         __builtin_amdgcn_sched_barrier(0);

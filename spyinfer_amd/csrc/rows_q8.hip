@@ -55,16 +55,41 @@ __device__ __forceinline__ RowScale row_scale(double a, double ss, float eps, in
     return {a > 0x1p-90 && a < 0x1p120 ? (float)(127.0 / a) : NAN, a, (float)(NORM ? scale / sqrt(ss / (double)H + (double)eps) : scale)};
 }
 
-// VEC values of a row in 16-byte pieces (8: the row is aligned so), or one.
+// VEC values of a row in one or two pieces, which are aligned so (VEC 8: 16 bytes each; 4: 16 or 8; 2: 8 or 4), or one value.
 template <int VEC, typename T>
 __device__ __forceinline__ void load_values(const T* p, float (&v)[VEC]) {
     if constexpr (VEC == 1) v[0] = to_f32<T>(*p);
+    else if constexpr (VEC == 2 && sizeof(T) == 4) { const float2 t = *reinterpret_cast<const float2*>(p); v[0] = t.x; v[1] = t.y; }
+    else if constexpr (VEC == 2) { const uint32_t t = *reinterpret_cast<const uint32_t*>(p); v[0] = __uint_as_float(t << 16); v[1] = __uint_as_float(t & 0xffff0000u); }
+    else if constexpr (VEC == 4) Vec4<T>::load(p, v);
     else if constexpr (sizeof(T) == 4) { Vec4<float>::load(p, v); Vec4<float>::load(p + 4, v + 4); }
     else {
         const uint4 t = *reinterpret_cast<const uint4*>(p);
         const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(w[e] << 16); v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+    }
+}
+// the stream's new values, and a row's integers
+template <int VEC>
+__device__ __forceinline__ void store_stream(float* p, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) *p = v[0];
+    else if constexpr (VEC == 2) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    else {
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) Vec4<float>::store(p + e, v + e);
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void store_integers(int8_t* o, const int (&n)[VEC]) {
+    if constexpr (VEC == 1) *o = (int8_t)n[0];
+    else if constexpr (VEC == 2) *reinterpret_cast<uint16_t*>(o) = (uint16_t)((n[0] & 255) | (n[1] & 255) << 8);
+    else {
+        uint32_t b[VEC / 4];
+#pragma unroll
+        for (int h = 0; h < VEC / 4; ++h) b[h] = (n[4 * h] & 255) | (n[4 * h + 1] & 255) << 8 | (n[4 * h + 2] & 255) << 16 | (uint32_t)n[4 * h + 3] << 24;
+        if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(o) = b[0];
+        else *reinterpret_cast<uint2*>(o) = uint2{b[0], b[1]};
     }
 }
 
@@ -100,8 +125,7 @@ __global__ __launch_bounds__(THREADS) void rows_q8_kernel(int8_t* __restrict__ q
             if (i < H) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[p][e] += d[p][e];
-                if constexpr (VEC == 1) s[i] = from_f32<TX>(v[p][0]);
-                else { Vec4<float>::store((float*)s + i, v[p]); Vec4<float>::store((float*)s + i + 4, v[p] + 4); }
+                store_stream<VEC>((float*)s + i, v[p]);
             }
         }
     }
@@ -127,14 +151,7 @@ __global__ __launch_bounds__(THREADS) void rows_q8_kernel(int8_t* __restrict__ q
         int n[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) n[e] = k.inv == 0.f ? 0 : quotient<NORM>(v[p][e], w[p][e], k.inv, k.a);
-        int8_t* o = q + row * pitch + i;
-        if constexpr (VEC == 1) *o = (int8_t)n[0];
-        else {
-            uint32_t b[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) b[h] = (n[4 * h] & 255) | (n[4 * h + 1] & 255) << 8 | (n[4 * h + 2] & 255) << 16 | (uint32_t)n[4 * h + 3] << 24;
-            *reinterpret_cast<uint2*>(o) = uint2{b[0], b[1]};
-        }
+        store_integers<VEC>(q + row * pitch + i, n);
     }
 }
 
@@ -164,21 +181,37 @@ __global__ __launch_bounds__(1024) void wide_rows_q8_kernel(int8_t* __restrict__
 template <typename TX, typename TD, typename TW, bool NORM>
 static void rows_launch(int8_t* q, float* scales, TX* x, int64_t ldx, const TD* delta, const TW* weight, float eps, int T, int H, int64_t pitch, hipStream_t st) {
 #define ROWS(VEC, THREADS, NP) rows_q8_kernel<TX, TD, TW, NORM, VEC, THREADS, NP><<<T, THREADS, 0, st>>>(q, scales, x, ldx, delta, weight, eps, H, pitch)
-    const bool vec = H % 8 == 0 && ldx % (16 / sizeof(TX)) == 0 && (((uintptr_t)x | (uintptr_t)delta | (uintptr_t)weight) % 16) == 0;
+    // pieces of eight values where every row begins at a multiple of 16 bytes, of four or two where it begins at one of theirs
+    const uintptr_t ends = (uintptr_t)x | (uintptr_t)delta | (uintptr_t)weight;
     const bool few = T <= 512;               // (blocks for all compute units are there anyway, or a thread has as little to do as possible)
-    if (vec && H <= 512) ROWS(8, 64, 1);
-    else if (vec && H <= 2048) ROWS(8, 256, 1);
-    else if (vec && H <= 4096) { if (few) ROWS(8, 512, 1); else ROWS(8, 256, 2); }
-    else if (vec && H <= 8192 && few) ROWS(8, 1024, 1);
-    else if (vec && H <= 6144) ROWS(8, 256, 3);
-    else if (vec && H <= 8192) ROWS(8, 512, 2);
-    else if (vec && H <= 16384 && few) ROWS(8, 1024, 2);
-    else if (vec && H <= 12288) ROWS(8, 512, 3);
-    else if (vec && H <= 16384) ROWS(8, 512, 4);
-    else if (vec && H <= 24576) ROWS(8, 1024, 3);
-    else if (vec && H <= 32768) ROWS(8, 1024, 4);
+    if (H % 8 == 0 && ldx % 8 == 0 && ends % 16 == 0 && H <= (NORM ? 16384 : 32768)) {
+        if (H <= 512) ROWS(8, 64, 1);
+        else if (H <= 2048) ROWS(8, 256, 1);
+        else if (H <= 4096) { if (few) ROWS(8, 512, 1); else ROWS(8, 256, 2); }
+        else if (H <= 8192 && few) ROWS(8, 1024, 1);
+        else if (H <= 6144) ROWS(8, 256, 3);
+        else if (H <= 8192) ROWS(8, 512, 2);
+        else if (H <= 16384 && few) ROWS(8, 1024, 2);
+        else if (H <= 12288) ROWS(8, 512, 3);
+        else if (H <= 16384) ROWS(8, 512, 4);
+        else if constexpr (!NORM) { if (H <= 24576) ROWS(8, 1024, 3); else ROWS(8, 1024, 4); }       // (a norm's registers would not do)
+    } else if (H % 4 == 0 && ldx % 4 == 0 && ends % 16 == 0 && H <= 16384) {
+        if (H <= 1024) ROWS(4, 256, 1);
+        else if (H <= 2048) ROWS(4, 256, 2);
+        else if (H <= 4096) { if (few) ROWS(4, 1024, 1); else ROWS(4, 256, 4); }
+        else if (H <= 8192) ROWS(4, 1024, 2);
+        else ROWS(4, 1024, 4);
+    } else if (H % 2 == 0 && ldx % 2 == 0 && ends % 8 == 0 && H <= 16384) {
+        if (H <= 512) ROWS(2, 256, 1);
+        else if (H <= 2048) ROWS(2, 256, 4);
+        else if (H <= 4096) { if (few) ROWS(2, 1024, 2); else ROWS(2, 256, 8); }
+        else ROWS(2, 1024, 8);
+    }
+    else if (H <= 256) ROWS(1, 256, 1);
     else if (H <= 1024) ROWS(1, 256, 4);
-    else if (H <= 4096) ROWS(1, 1024, 4);
+    else if (H <= 2048) ROWS(1, 256, 8);
+    else if (H <= 4096) { if (few) ROWS(1, 1024, 4); else ROWS(1, 256, 16); }
+    else if (H <= 8192) ROWS(1, 1024, 8);
     else if (H <= 16384) ROWS(1, 1024, 16);
     else wide_rows_q8_kernel<TX, TD, TW, NORM><<<T, 1024, 0, st>>>(q, scales, x, ldx, delta, weight, eps, H, pitch);
 #undef ROWS

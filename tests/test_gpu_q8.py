@@ -43,7 +43,7 @@ def uneven(shape, seed, dtype=torch.float32):
     return x.to(dtype)
 
 
-SIZES = [(1, 1), (3, 2), (1, 4096), (2, 17), (5, 64), (7, 1001), (61, 250), (9, 1024), (4, 5120), (3, 12288), (2, 20480), (130, 96), (257, 4096), (1025, 128), (300, 2560), (2, 130816)]
+SIZES = [(1, 1), (3, 2), (1, 4096), (2, 17), (5, 64), (7, 1001), (61, 250), (9, 1024), (4, 5120), (3, 12288), (2, 20480), (130, 96), (9, 1084), (3, 2830), (700, 1548), (600, 3001), (520, 2050), (2, 6226), (4, 16796), (3, 16398), (600, 5120), (530, 12288), (2, 24576), (1, 32768), (257, 4096), (1025, 128), (300, 2560), (2, 130816)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
