@@ -16,6 +16,6 @@ __device__ __forceinline__ void q8_store_piece(bf16_t* o, const float (&v)[8]) {
 }
 __device__ __forceinline__ void q8_store_piece(float* o, const float (&v)[4]) { *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]); }
 
-// Blocks of MT (8 to 16) row tiles and 256 columns, one a compute unit (gemm_q8_tall.hip)
-int q8_tall_launch(void* C, int c_dtype, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int gated,
+// Blocks of MT (8 to 16) row tiles and 256 columns, one a compute unit (gemm_q8_tall.hip); M >= 16 MT
+int q8_tall_launch(void* C, int c_dtype, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int gated,
                    GateAct act, int MT, hipStream_t st);

@@ -39,8 +39,8 @@ __device__ __forceinline__ void q8_wait_loads() {
 
 // ONCE: W is read by one block only, and passes the caches by (up to 64 rows, matrices from memory: 16 rows, 4096 -> 2 x 12288 19.8 / 18.4 us).
 template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename TC>
-__device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks,
-                                                int n_rows, int blocks, const GateAct& act) {
+__device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int n_rows,
+                                                int blocks, const GateAct& act) {
     constexpr int PAIR = EPI == Q8_GATED ? 2 : 1, NO = NT / PAIR, PIECES = 4 * S, RPI = 16 / S;            // pieces of a row, rows that a load brings
     constexpr int ITEMS = MT * NO, MOST = MT * S / PAIR, PHASE = ITEMS < MOST ? ITEMS : MOST, OPS = MT * S + NT * S;
     static_assert(D >= 2 && D <= 3 && (D - 1) * OPS <= 63, "a wait counts the loads issued after those that it waits for");
@@ -61,32 +61,36 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, int64_t 
         const int n = tid - MT * 16, tile = col0 + n / 16 % NO;
         if (tile < tiles / PAIR) scale = sw[(n / 16 / NO * (tiles / PAIR) + tile) * 16 + n % 16];
     }
-    const int w_bytes = tiles * chunks * 4096, x_bytes = (int)(rows * pitch), n_units = chunks * 4 / S;
+    const int w_bytes = tiles * chunks * 4096, pitch = chunks * Q8_CHUNK, n_units = chunks * 4 / S;
     const auto wres = __builtin_amdgcn_make_buffer_rsrc((void*)W, 0, w_bytes, 0x00020000);
-    const auto xres = __builtin_amdgcn_make_buffer_rsrc((void*)(X + row0 * pitch), 0, x_bytes, 0x00020000);
+    const auto xres = __builtin_amdgcn_make_buffer_rsrc((void*)(X + (size_t)row0 * pitch), 0, rows * pitch, 0x00020000);
     int w_at[NT], x_lane[S];
 #pragma unroll
     for (int j = 0; j < NT; ++j) w_at[j] = min(col0 + j % NO, tiles / PAIR - 1) * 4096 + j / NO * (tiles / PAIR) * 4096;
 #pragma unroll
-    for (int q = 0; q < S; ++q) x_lane[q] = (q * RPI + lane / PIECES) * (int)pitch + (lane % PIECES ^ (q * RPI + lane / PIECES) * S / 4) * 16;
+    for (int q = 0; q < S; ++q) x_lane[q] = (q * RPI + lane / PIECES) * pitch + (lane % PIECES ^ (q * RPI + lane / PIECES) * S / 4) * 16;
     q8_i32x4_t acc[NT][MT], w[D][S][NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = q8_i32x4_t{0, 0, 0, 0};
     char* const mine[3] = {stage0 + wave * MT * S * 1024, stage1 + wave * MT * S * 1024, stage2 + (D > 2 ? wave * MT * S * 1024 : 0)};
+    // A lane's own offset alone says whether a load lies in its buffer (the offset that all lanes share may not count): rows that do not exist, and whatever
+    // belongs to a unit behind the end, lie beyond (2^30 is more than any block's rows, 2^31 more than any matrix)
     auto load = [&](int d, int unit) {
         const bool some = unit < n_units;
-        const int wo = some ? (unit * S >> 2) * tiles * 4096 + (unit * S & 3) * 1024 : w_bytes, xo = some ? unit * S * Q8_STEP : x_bytes;
+        const int wo = some ? (unit * S >> 2) * tiles * 4096 + (unit * S & 3) * 1024 : 0, xo = some ? unit * S * Q8_STEP : 0;
+        const unsigned w_lane = some ? lane * 16 : 0x80000000u;
+        const int x_skip = some ? 0 : 1 << 30;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int q = 0; q < S; ++q)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (__attribute__((address_space(3))) void*)(mine[d] + (i * S + q) * 1024), 16, x_lane[q], xo + i * 16 * (int)pitch, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (__attribute__((address_space(3))) void*)(mine[d] + (i * S + q) * 1024), 16, x_lane[q] + (i * 16 * pitch + x_skip), xo, 0, 0);
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) w[d][s][j] = __builtin_bit_cast(q8_i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(wres, lane * 16, w_at[j] + wo + s * 1024, ONCE ? 2 : 0));
+            for (int j = 0; j < NT; ++j) w[d][s][j] = __builtin_bit_cast(q8_i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(wres, w_lane, w_at[j] + wo + s * 1024, ONCE ? 2 : 0));
         __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
@@ -139,13 +143,13 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, int64_t 
 }
 
 template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename TC>
-__global__ __launch_bounds__(WAVES * 64) void gemm_q8_kernel(TC* C, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N,
+__global__ __launch_bounds__(WAVES * 64) void gemm_q8_kernel(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N,
                                                                     int tiles, int chunks, int n_rows, int blocks, GateAct act) {
-    q8_staged_block<WAVES, MT, NT, S, D, ONCE, EPI, TC>(C, X, pitch, sx, W, sw, M, N, tiles, chunks, n_rows, blocks, act);
+    q8_staged_block<WAVES, MT, NT, S, D, ONCE, EPI, TC>(C, X, sx, W, sw, M, N, tiles, chunks, n_rows, blocks, act);
 }
 
 struct Q8Args {
-    void* C; int c_dtype; const int8_t* X; int64_t pitch; const float* sx; const int8_t* W; const float* sw; int M, N, tiles, chunks, gated; GateAct act; hipStream_t st;
+    void* C; int c_dtype; const int8_t* X; const float* sx; const int8_t* W; const float* sw; int M, N, tiles, chunks, gated; GateAct act; hipStream_t st;
 };
 
 template <int MT, int NT, int S, int D>
@@ -155,7 +159,7 @@ static int split_launch(const Q8Args& a) {
     const int64_t blocks = (int64_t)n_rows * n_cols;
     SPY_REQUIRE(blocks < (1 << 30), "spy_gemm_q8: %lld blocks", (long long)blocks);
     const unsigned grid = (unsigned)((blocks + Q8_DIES - 1) / Q8_DIES * Q8_DIES);
-#define SPLIT_ARGS(TC) (TC*)a.C, a.X, a.pitch, a.sx, a.W, a.sw, a.M, a.N, a.tiles, a.chunks, n_rows, (int)blocks, a.act
+#define SPLIT_ARGS(TC) (TC*)a.C, a.X, a.sx, a.W, a.sw, a.M, a.N, a.tiles, a.chunks, n_rows, (int)blocks, a.act
 #define SPLIT_BY(ONCE, EPI, TC) gemm_q8_kernel<4, MT, NT, S, D, ONCE, EPI, TC><<<grid, 256, 0, a.st>>>(SPLIT_ARGS(TC))
     // (more than four row tiles, or four column tiles, are for products of more rows)
 #define SPLIT(EPI, TC) do { if (n_rows == 1 && MT <= 4 && NT <= 2) SPLIT_BY((MT <= 4 && NT <= 2), EPI, TC); else SPLIT_BY(false, EPI, TC); } while (0)
@@ -190,8 +194,8 @@ static int q8_plan(int M, int tiles, int chunks, int gated) {
     for (const Q8Cost& p : q8_costs) {
         const bool tall = p.plan < 100;
         const int MT = tall ? p.plan : p.plan % 100, NO = tall ? (gated ? 8 : 16) : p.plan / 100 / (gated ? 2 : 1);
-        // not many more row tiles than there are (four from 33 rows on, six from 81, eight from 113, tall from 65)
-        if (NO < 1 || (tall ? M <= 64 : MT == 4 ? row_tiles < 3 : row_tiles < MT)) continue;
+        // not many more row tiles than there are (four from 33 rows on, six from 81, eight from 113), tall blocks no more
+        if (NO < 1 || (tall ? M < 16 * MT : MT == 4 ? row_tiles < 3 : row_tiles < MT)) continue;
         const int cols = (col_tiles + NO - 1) / NO;
         const float blocks = (float)((row_tiles + MT - 1) / MT) * (float)cols / 256.f, rounds = ceilf(blocks), k = (float)chunks;
         const float us = p.c[0] + p.c[1] * rounds * k + p.c[2] * rounds + p.c[3] * blocks * k + p.c[4] * (tall ? blocks : (float)row_tiles * cols / 256.f * k);
@@ -200,21 +204,20 @@ static int q8_plan(int M, int tiles, int chunks, int gated) {
     return best;
 }
 
-// C: bfloat16 or float32 [M, N].  X: rows of `pitch` bytes (a multiple of 16) and their scales; W: the matrix laid out, `tiles` column tiles (gated:
+// C: bfloat16 or float32 [M, N].  X: rows of 256 bytes a chunk and their scales; W: the matrix laid out, `tiles` column tiles (gated:
 // of both halves) and `chunks` of K, and its scales [16 tiles].  Gated: C is bfloat16 [M, N], N one half's columns.
 // plan: 0, or the blocks by name (q8_costs).
-extern "C" int spy_gemm_q8(void* C, int c_dtype, const void* X, int64_t pitch, const float* sx, const void* W, const float* sw, int M, int N, int tiles, int chunks,
+extern "C" int spy_gemm_q8(void* C, int c_dtype, const void* X, const float* sx, const void* W, const float* sw, int M, int N, int tiles, int chunks,
                            int gated, int act_code, int plan, hipStream_t st) {
     GateAct act = {1.f, 0.f};
     SPY_REQUIRE(M > 0 && N > 0 && tiles > 0 && chunks > 0, "spy_gemm_q8: empty operand");
-    SPY_REQUIRE(pitch % 16 == 0 && pitch <= (int64_t)chunks * Q8_CHUNK && pitch > (int64_t)(chunks - 1) * Q8_CHUNK, "spy_gemm_q8: rows of %lld bytes for %d chunks of K", (long long)pitch, chunks);
     SPY_REQUIRE(chunks <= 511 && (int64_t)tiles * chunks * 4096 < (1ll << 31), "spy_gemm_q8: a matrix of %d x %d tiles is too large", tiles, chunks);
     SPY_REQUIRE(gated ? tiles % 2 == 0 && N <= tiles * 8 && N > tiles * 8 - 16 : N <= tiles * 16 && N > tiles * 16 - 16, "spy_gemm_q8: %d columns in %d tiles", N, tiles);
     SPY_REQUIRE((((uintptr_t)X | (uintptr_t)W) % 16) == 0, "spy_gemm_q8: operands must be 16-byte aligned");
     SPY_REQUIRE(!gated || (gate_act_of(act_code, &act) && c_dtype == SPY_BF16), "spy_gemm_q8: activation %d, result dtype %d", act_code, c_dtype);
-    const Q8Args a = {C, c_dtype, (const int8_t*)X, pitch, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, st};
+    const Q8Args a = {C, c_dtype, (const int8_t*)X, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, st};
     if (!plan) plan = q8_plan(M, tiles, chunks, gated);
-    if (plan >= 8 && plan <= 16) return q8_tall_launch(C, c_dtype, (const int8_t*)X, pitch, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, plan, st);
+    if (plan >= 8 && plan <= 16) return q8_tall_launch(C, c_dtype, (const int8_t*)X, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, plan, st);
     switch (plan) {
         case 101: return split_launch<1, 1, 4, 2>(a);
         case 102: return split_launch<2, 1, 2, 3>(a);

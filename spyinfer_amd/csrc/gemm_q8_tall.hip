@@ -13,9 +13,9 @@ struct TallQ8 {
 
 // A block's results through its LDS stage, as many row tiles at a time as fit, in a part that a wave has to itself: the sums go there as they are, and a short loop reads
 // pieces of rows, forms the values and stores whole lines.  A piece of four columns lies at place p ^ (row % 16).
-// sx: the block's row scales in LDS; sw: the column scales, those of the up rows `half` on; at: this wave's first column; rows, columns: those that exist.
+// sx: the block's row scales in LDS; sw: the column scales, those of the up rows `half` on; at: this wave's first column; columns: those that exist.
 template <int MT, int EPI, typename TC>
-__device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t* stage, TC* out, int64_t ld, int rows, int columns, int at, const float* sx, const float* sw,
+__device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t* stage, TC* out, int64_t ld, int columns, int at, const float* sx, const float* sw,
                                                 int half, const GateAct& act, int lane, int wave) {
     constexpr int CT = MT / 4, VEC = 16 / sizeof(TC), PIECES = (EPI == Q8_GATED ? 32 : 64) / VEC, ROWS = 64 / PIECES;
     int* mine = reinterpret_cast<int*>(stage) + wave * CT * 16 * 64;
@@ -34,8 +34,8 @@ __device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t
 #pragma unroll
             for (int j = 0; j < 4; ++j) *reinterpret_cast<q8_i32x4_t*>(mine + ((i - i0) * 16 + r) * 64 + ((j * 4 + g) ^ r) * 4) = acc[j][i];
         __builtin_amdgcn_sched_barrier(0);
-        const int here = min(16 * min(CT, MT - i0), rows - i0 * 16);
-        if (whole || sizeof(TC) == 2) {
+        const int here = 16 * min(CT, MT - i0);
+        if (whole) {
 #pragma unroll 2
             for (int row = lane / PIECES; row < here; row += ROWS) {
                 const int* from = mine + row * 64;
@@ -49,22 +49,18 @@ __device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t
                     for (int e = 0; e < 4; ++e) v[k * 4 + e] = q8_value<EPI>(act, a[e], b[e], fx, fw[k * 4 + e], fu[k * 4 + e]);
                 }
                 TC* o = out + (int64_t)(i0 * 16 + row) * ld + column;
-                if (whole) { if (column < columns) q8_store_piece(o, v); }
-                else {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        if (column + e < columns) o[e] = from_f32<TC>(v[e]);
-                }
+                if (column < columns) q8_store_piece(o, v);
             }
         } else {
-            // float32 rows that begin anywhere: a lane has a column (of bfloat16 that is slower than single values of a piece: 2228 rows, 4096 -> 705 28.3 / 31.8 us)
-            const int c = lane;
+            // rows that begin anywhere: a lane has a column
+            constexpr int WIDTH = EPI == Q8_GATED ? 32 : 64;
+            const int c = lane % WIDTH, up = c + (EPI == Q8_GATED ? 32 : 0);
             const bool is = at + c < columns;
-            const float cw = is ? sw[at + c] : 0.f;
+            const float cw = is ? sw[at + c] : 0.f, cu = EPI == Q8_GATED && is ? sw[half + at + c] : 0.f;
 #pragma unroll 8
-            for (int row = 0; row < here; ++row) {
-                const int a = mine[row * 64 + ((c / 4) ^ (row & 15)) * 4 + c % 4];
-                if (is) out[(int64_t)(i0 * 16 + row) * ld + at + c] = from_f32<TC>(q8_value<Q8_STORE>(act, a, a, sx[i0 * 16 + row], cw, 0.f));
+            for (int row = lane / WIDTH; row < here; row += 64 / WIDTH) {
+                const int a = mine[row * 64 + ((c / 4) ^ (row & 15)) * 4 + c % 4], b = mine[row * 64 + ((up / 4) ^ (row & 15)) * 4 + up % 4];
+                if (is) out[(int64_t)(i0 * 16 + row) * ld + at + c] = from_f32<TC>(q8_value<EPI>(act, a, b, sx[i0 * 16 + row], cw, cu));
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -72,7 +68,7 @@ __device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t
 }
 
 template <int MT, int EPI, typename TC>
-__global__ __launch_bounds__(256, 1) void gemm_q8_tall_kernel(TC* C, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N,
+__global__ __launch_bounds__(256, 1) void gemm_q8_tall_kernel(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N,
                                                               int tiles, int chunks, int n_rows, int n_cols, int blocks, GateAct act) {
     __shared__ __align__(1024) bf16_t stage0[MT * 16 * 128];
     __shared__ __align__(1024) bf16_t stage1[MT * 16 * 128];
@@ -81,11 +77,12 @@ __global__ __launch_bounds__(256, 1) void gemm_q8_tall_kernel(TC* C, const int8_
     const int per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;
     const int v = (blockIdx.x % Q8_DIES) * per + idx;
     if (idx >= per || v >= blocks) return;
-    const int col_t = v / n_rows, row0 = (v % n_rows) * MT * 16, rows = min(M - row0, MT * 16);
+    const int col_t = v / n_rows, pitch = chunks * Q8_CHUNK;
+    const int row0 = min((v % n_rows) * MT * 16, M - MT * 16);          // the last rows' tile ends with row M - 1 (what it shares with the one before, both form alike)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if ((int)threadIdx.x < rows) row_scales[threadIdx.x] = sx[row0 + threadIdx.x];              // (MT <= 16; behind the turns' barriers when it is read)
+    if (threadIdx.x < MT * 16) row_scales[threadIdx.x] = sx[row0 + threadIdx.x];              // (MT <= 16; behind the turns' barriers when it is read)
     const auto wres = __builtin_amdgcn_make_buffer_rsrc((void*)W, 0, tiles * chunks * 4096, 0x00020000);
-    const auto xres = __builtin_amdgcn_make_buffer_rsrc((void*)(X + row0 * pitch), 0, (int)(rows * pitch), 0x00020000);       // (what lies behind reads as zeros)
+    const auto xres = __builtin_amdgcn_make_buffer_rsrc((void*)(X + (size_t)row0 * pitch), 0, MT * 16 * pitch, 0x00020000);
     int w_at[4];                                       // this wave's column tiles; one that does not exist reads the last (nothing is stored)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -94,24 +91,24 @@ __global__ __launch_bounds__(256, 1) void gemm_q8_tall_kernel(TC* C, const int8_
     }
     // X: a wave's load brings 4 rows of 256 bytes; lane l has the piece that belongs to place l % 16 of row l / 16
     const int s_row = wave * 4 + (lane >> 4);
-    const int x_lane = s_row * (int)pitch + ((lane & 15) ^ s_row) * 16;
+    const int x_lane = s_row * pitch + ((lane & 15) ^ s_row) * 16;
     q8_i32x4_t acc[4][MT];
     gr_tall_turns<TallQ8, MT>(acc, wres, lane * 16, w_at, tiles * 4096, chunks, stage0, stage1, lane, [&](bf16_t* stage, int i, int c) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (__attribute__((address_space(3))) void*)(stage + (i * 4 + wave) * 512), 16, x_lane,
-                                                 i * 16 * (int)pitch + c * Q8_CHUNK, 0, 0);
+                                                 i * 16 * pitch + c * Q8_CHUNK, 0, 0);
     });
     constexpr int WAVE_COLUMNS = EPI == Q8_GATED ? 32 : 64;
-    q8_tall_results<MT, EPI, TC>(acc, stage0, C + (size_t)row0 * N, N, rows, N, (col_t * 4 + wave) * WAVE_COLUMNS, row_scales, sw, tiles * 8, act, lane, wave);
+    q8_tall_results<MT, EPI, TC>(acc, stage0, C + (size_t)row0 * N, N, N, (col_t * 4 + wave) * WAVE_COLUMNS, row_scales, sw, tiles * 8, act, lane, wave);
 }
 
 template <int MT>
-static int tall_launch(void* C, int c_dtype, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int gated,
+static int tall_launch(void* C, int c_dtype, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int gated,
                        GateAct act, hipStream_t st) {
     const int n_rows = (M + MT * 16 - 1) / (MT * 16), n_cols = gated ? (N + 127) / 128 : (N + 255) / 256;
     const int64_t blocks = (int64_t)n_rows * n_cols;
-    SPY_REQUIRE(blocks < (1 << 30), "spy_gemm_q8: %lld blocks", (long long)blocks);
+    SPY_REQUIRE(M >= MT * 16 && blocks < (1 << 30), "spy_gemm_q8: %d rows in blocks of %d row tiles, %lld blocks", M, MT, (long long)blocks);
     const unsigned grid = (unsigned)((blocks + Q8_DIES - 1) / Q8_DIES * Q8_DIES);
-#define TALL(EPI, TC) gemm_q8_tall_kernel<MT, EPI, TC><<<grid, 256, 0, st>>>((TC*)C, X, pitch, sx, W, sw, M, N, tiles, chunks, n_rows, n_cols, (int)blocks, act)
+#define TALL(EPI, TC) gemm_q8_tall_kernel<MT, EPI, TC><<<grid, 256, 0, st>>>((TC*)C, X, sx, W, sw, M, N, tiles, chunks, n_rows, n_cols, (int)blocks, act)
     if (gated) TALL(Q8_GATED, bf16_t);
     else if (c_dtype == SPY_F32) TALL(Q8_STORE, float);
     else TALL(Q8_STORE, bf16_t);
@@ -120,9 +117,9 @@ static int tall_launch(void* C, int c_dtype, const int8_t* X, int64_t pitch, con
     return 0;
 }
 
-int q8_tall_launch(void* C, int c_dtype, const int8_t* X, int64_t pitch, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int gated,
+int q8_tall_launch(void* C, int c_dtype, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int gated,
                    GateAct act, int MT, hipStream_t st) {
-#define CASE(T) case T: return tall_launch<T>(C, c_dtype, X, pitch, sx, W, sw, M, N, tiles, chunks, gated, act, st)
+#define CASE(T) case T: return tall_launch<T>(C, c_dtype, X, sx, W, sw, M, N, tiles, chunks, gated, act, st)
     switch (MT) { CASE(8); CASE(10); CASE(12); CASE(14); CASE(16); }
 #undef CASE
     return spy_fail("spy_gemm_q8: %d row tiles", MT);

@@ -1,7 +1,7 @@
 // Rows and matrices in 8-bit integers.
 //
-// Rows: int8 [rows][pitch], pitch = the width rounded up to 16 (what lies behind a row's last value is never read for a result: the matrix
-// has zeros there), and a float32 scale for each row; a row stands for integers times its scale.
+// Rows: int8 [rows][pitch], pitch = the width rounded up to 256 (what lies behind a row's last value may be anything: the matrix has zeros there), and a
+// float32 scale for each row; a row stands for integers times its scale.
 // Matrices: [K/256 chunks][N/16 tiles][4 steps][64 lanes][16 bytes], lane 16 g + r of step s of chunk c of tile t holding
 // W[16 t + r][256 c + 64 s + 16 g ..]: a wave's operand of one 16 x 16 x 64 product is one load of 1 KiB in one piece.  K is filled up to 256 and N to 16
 // with zeros (a gated matrix' gate rows and up rows each), and every row of W has a float32 scale.

@@ -95,7 +95,7 @@ class _Hip:
         # ctypes object per argument: 3 us of the host's 14 per call)
         P, I = ctypes.c_void_p, ctypes.c_int
         self.lib.spy_gemm_decode.argtypes = [P, I, P, I, ctypes.c_float, P, I, P, I, P, P, P, P, I, I, I, I, I, I, P, ctypes.c_int64, I, P]
-        self.lib.spy_gemm_q8.argtypes = [P, I, P, ctypes.c_int64, P, P, P, I, I, I, I, I, I, I, P]
+        self.lib.spy_gemm_q8.argtypes = [P, I, P, P, P, P, I, I, I, I, I, I, I, P]
         self.lib.spy_add_rmsnorm_q8.argtypes = [P, P, P, P, I, P, I, ctypes.c_float, I, I, ctypes.c_int64, P]
         self.lib.spy_quantize_rows.argtypes = [P, P, P, I, ctypes.c_int64, I, I, ctypes.c_int64, P]
 
@@ -2738,12 +2738,12 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 
 class Q8Rows:
     """Rows in 8-bit integers: row t stands for ``values[t, :width]`` times ``scales[t]``.  ``values`` int8 [T, pitch], dense, pitch the
-    width rounded up to 16 (what lies behind a row's end is anything); ``scales`` float32 [T]."""
+    width rounded up to 256 (what lies behind a row's end is anything); ``scales`` float32 [T]."""
     __slots__ = ("values", "scales", "width")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, width: int):
-        _check(values.dtype == torch.int8 and values.dim() == 2 and width > 0 and values.shape[1] == (width + 15) & -16 and values.is_contiguous()
-               and values.data_ptr() % 16 == 0, "Q8Rows: dense int8 values [T, width rounded up to 16] expected")
+        _check(values.dtype == torch.int8 and values.dim() == 2 and width > 0 and values.shape[1] == (width + 255) & -256 and values.is_contiguous()
+               and values.data_ptr() % 16 == 0, "Q8Rows: dense int8 values [T, width rounded up to 256] expected")
         _check(tuple(scales.shape) == (values.shape[0],) and scales.dtype == torch.float32 and scales.is_contiguous() and scales.device == values.device,
                "Q8Rows: a float32 scale for each row expected")
         self.values, self.scales, self.width = values, scales, width
@@ -2756,8 +2756,8 @@ class Q8Rows:
         """``values`` int8 [T, K] with a scale for each row, float32 [T]."""
         _check(values.dim() == 2 and values.dtype == torch.int8 and values.shape[1] > 0, "Q8Rows: int8 values [T, K] expected")
         T, K = values.shape
-        if K % 16 or not values.is_contiguous() or values.data_ptr() % 16:
-            kept = torch.zeros((T, (K + 15) & -16), dtype=torch.int8, device=values.device)
+        if K % 256 or not values.is_contiguous() or values.data_ptr() % 16:
+            kept = torch.zeros((T, (K + 255) & -256), dtype=torch.int8, device=values.device)
             kept[:, :K] = values
             values = kept
         return Q8Rows(values, scales, K)
@@ -2770,7 +2770,7 @@ class Q8Rows:
 def _new_q8_rows(like: torch.Tensor, T: int, width: int) -> Q8Rows:
     """Rows to be written, on the device of ``like`` (made without the constructor's checks: a step has hundreds)."""
     rows = Q8Rows.__new__(Q8Rows)
-    rows.values, rows.scales, rows.width = like.new_empty((T, (width + 15) & -16), dtype=torch.int8), like.new_empty((T,), dtype=torch.float32), width
+    rows.values, rows.scales, rows.width = like.new_empty((T, (width + 255) & -256), dtype=torch.int8), like.new_empty((T,), dtype=torch.float32), width
     return rows
 
 
@@ -2853,7 +2853,7 @@ def quantize_rows(x: torch.Tensor) -> Q8Rows:
             return quantize_rows(x)
     rows = _new_q8_rows(x, T, K)
     if T:
-        hip().call("spy_quantize_rows", rows.values.data_ptr(), rows.scales.data_ptr(), x.data_ptr(), code, ld if T > 1 else K, T, K, (K + 15) & -16,
+        hip().call("spy_quantize_rows", rows.values.data_ptr(), rows.scales.data_ptr(), x.data_ptr(), code, ld if T > 1 else K, T, K, (K + 255) & -256,
                    _raw_stream(device))
     return rows
 
@@ -2882,7 +2882,7 @@ def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
     rows = _new_q8_rows(resid, T, H)
     if T:
         hip().call("spy_add_rmsnorm_q8", rows.values.data_ptr(), rows.scales.data_ptr(), resid.data_ptr(), None if delta is None else delta.data_ptr(), delta_code,
-                   weight.data_ptr(), weight_code, eps, T, H, (H + 15) & -16, _raw_stream(device))
+                   weight.data_ptr(), weight_code, eps, T, H, (H + 255) & -256, _raw_stream(device))
     return rows
 
 
@@ -2898,10 +2898,10 @@ def _gemm_q8(name: str, x: Q8Rows, w: Q8Weight, out_dtype: torch.dtype, out: Opt
     if device != _current_device():
         with torch.cuda.device(device):
             return _gemm_q8(name, x, w, out_dtype, out, columns, act)
-    T, pitch = values.shape
+    T = values.shape[0]
     out = values.new_empty((T, columns), dtype=out_dtype) if out is None else _result(out, T, columns, out_dtype, values.device)
     if T:
-        hip().call("spy_gemm_q8", out.data_ptr(), _CODES[out_dtype], values.data_ptr(), pitch, x.scales.data_ptr(), tiles.data_ptr(), w.scales.data_ptr(), T, columns,
+        hip().call("spy_gemm_q8", out.data_ptr(), _CODES[out_dtype], values.data_ptr(), x.scales.data_ptr(), tiles.data_ptr(), w.scales.data_ptr(), T, columns,
                    tiles.shape[1], tiles.shape[0], 1 if w.gated else 0, act, Q8_PLAN, _raw_stream(device))
     return out
 

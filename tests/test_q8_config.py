@@ -45,7 +45,7 @@ def test_binding(monkeypatch):
 
 def test_products_go_by_the_matrix(monkeypatch):
     """Every product of a part takes a matrix in 8 bits in a matrix' place, and rows in 8 bits or not."""
-    rows, w, wg = (ops.Q8Rows(torch.zeros((2, 16), dtype=torch.int8), torch.ones(2), 16), ops.Q8Weight.from_values(torch.zeros((8, 16), dtype=torch.int8), torch.ones(8)),
+    rows, w, wg = (ops.Q8Rows(torch.zeros((2, 256), dtype=torch.int8), torch.ones(2), 16), ops.Q8Weight.from_values(torch.zeros((8, 16), dtype=torch.int8), torch.ones(8)),
                    ops.Q8Weight.from_values(torch.zeros((8, 16), dtype=torch.int8), torch.ones(8), gated=True))
     calls = []
     monkeypatch.setattr(ops, "quantize_rows", lambda x: rows)

@@ -7,7 +7,7 @@ from spyinfer_amd.kernels.ops import KernelError, Q8Rows, Q8Weight
 
 
 def rows(t=2, k=32):
-    return Q8Rows(torch.zeros((t, (k + 15) // 16 * 16), dtype=torch.int8), torch.ones(t), k)
+    return Q8Rows(torch.zeros((t, (k + 255) // 256 * 256), dtype=torch.int8), torch.ones(t), k)
 
 
 def weight(n=32, k=32, gated=False):
@@ -29,10 +29,10 @@ def weight(n=32, k=32, gated=False):
     (lambda: ops.linear_q8_gated(rows(), weight(gated=True), "relu"), "relu"),
     (lambda: ops.linear_q8_gated(rows(), weight(gated=True)), "GPU only"),
     (lambda: ops.quantize_weight(torch.zeros(4, 8)), "on the GPU"),
-    (lambda: Q8Rows(torch.zeros((2, 33), dtype=torch.int8), torch.ones(2), 33), "rounded up to 16"),
-    (lambda: Q8Rows(torch.zeros((2, 48), dtype=torch.int8), torch.ones(2), 32), "rounded up to 16"),
-    (lambda: Q8Rows(torch.zeros((48, 2), dtype=torch.int8).t(), torch.ones(2), 48), "dense"),
-    (lambda: Q8Rows(torch.zeros((2, 48), dtype=torch.int8), torch.ones(4)[::2], 48), "scale"),
+    (lambda: Q8Rows(torch.zeros((2, 33), dtype=torch.int8), torch.ones(2), 33), "rounded up to 256"),
+    (lambda: Q8Rows(torch.zeros((2, 512), dtype=torch.int8), torch.ones(2), 256), "rounded up to 256"),
+    (lambda: Q8Rows(torch.zeros((256, 2), dtype=torch.int8).t(), torch.ones(2), 48), "dense"),
+    (lambda: Q8Rows(torch.zeros((2, 256), dtype=torch.int8), torch.ones(4)[::2], 48), "scale"),
     (lambda: Q8Weight(torch.zeros((1, 2, 4, 4, 16, 16), dtype=torch.int8), torch.ones(16), (32, 256), False), "scale"),
     (lambda: Q8Weight(torch.zeros((1, 2, 4, 4, 16, 16), dtype=torch.int8), torch.ones(32), (33, 256), False), "tiles"),
     (lambda: Q8Weight(torch.zeros((1, 2, 4, 4, 16, 16), dtype=torch.int8), torch.ones(32), (31, 256), True), "gate and up"),
@@ -64,9 +64,9 @@ def test_a_matrix_laid_out_is_the_matrix(N, K, gated):
             assert w.tiles[k // 256, row // 16, k // 64 % 4, k // 16 % 4, row % 16, k % 16] == p[n, k]
 
 
-def test_rows_of_any_width_are_kept_in_pieces_of_16():
+def test_rows_of_any_width_are_kept_in_pieces_of_256():
     q = torch.arange(-33, 33, dtype=torch.int8).view(2, 33)
-    r = Q8Rows(torch.zeros((2, 48), dtype=torch.int8), torch.tensor([2.0, 0.5]), 33)
+    r = Q8Rows(torch.zeros((2, 256), dtype=torch.int8), torch.tensor([2.0, 0.5]), 33)
     r.values[:, :33] = q
     assert torch.equal(r.to_rows(), q.float() * r.scales[:, None]) and r.shape == (2, 33)
 
