@@ -35,24 +35,23 @@ __device__ __forceinline__ void row_statistics(BITS& top, double& ss) {
     for (int i = 1; i < WAVES; ++i) { top = max(top, tops[i]); if (SUM) ss += sums[i]; }
 }
 
-// 127 z / a rounded half to even, z = x or x w.  In 32 bits the quotient is off by up to 3 2^-24 of 127 (the product, 127 / a and theirs), less than 2^-15; adding
+// 127 z / a rounded half to even, z = x or x w.  In 32 bits the quotient is off by up to 4 2^-24 of 127 (the product, a, 127 / a and theirs), less than 2^-15; adding
 // 1.5 2^23 leaves its nearest integer in the low bits, and only where what that leaves out is half an integer, but for 2^-15, is the quotient itself formed, in 64 bits (one value
-// of 16 000, and ties).  Rows whose largest value is very large or small, for which 127 / a has no 32 bits, go by that altogether (inv NaN).
+// of 16 000, and ties).  Rows whose largest value is very large or small, for which 127 / a has no 32 bits, go by that altogether (inv NaN); rows
+// whose integers are all 0 have inv 0.
 template <bool NORM>
 __device__ __forceinline__ int quotient(float x, float w, float inv, double a) {
     const float u = (NORM ? x * w : x) * inv, t = u + 12582912.f;
     if (__builtin_expect(!(fabsf(u - (t - 12582912.f)) <= 0.5f - 0x1p-15f), 0)) return (int)rint((NORM ? (double)x * (double)w : (double)x) * 127.0 / a);
     return (int)__float_as_uint(t);
 }
+__device__ __forceinline__ float inverse(double a) { return !(a < INFINITY) || a == 0. ? 0.f : a > 0x1p-90 && a < 0x1p120 ? 127.f / (float)a : NAN; }
 
-// What a row's statistics make of it: 127 / a and a (0 and 1 where all integers are 0), and its scale.
-struct RowScale { float inv; double a; float scale; };
+// A row's scale from its largest magnitude and, for the norm, its sum of squares.
 template <bool NORM>
-__device__ __forceinline__ RowScale row_scale(double a, double ss, float eps, int H) {
-    if (!(a < INFINITY)) return {0.f, 1., NAN};
-    if (a == 0.) return {0.f, 1., 0.f};
-    const double scale = a / 127.0;
-    return {a > 0x1p-90 && a < 0x1p120 ? (float)(127.0 / a) : NAN, a, (float)(NORM ? scale / sqrt(ss / (double)H + (double)eps) : scale)};
+__device__ __forceinline__ float row_scale(double a, double ss, float eps, int H) {
+    if (!(a < INFINITY)) return NAN;
+    return (float)(a / (NORM ? 127.0 * sqrt(ss / (double)H + (double)eps) : 127.0));
 }
 
 // VEC values of a row in one or two pieces, which are aligned so (VEC 8: 16 bytes each; 4: 16 or 8; 2: 8 or 4), or one value.
@@ -142,17 +141,18 @@ __global__ __launch_bounds__(THREADS) void rows_q8_kernel(int8_t* __restrict__ q
             } else top = max(top, magnitude(v[p][e]));
         }
     row_statistics<THREADS / 64, NORM>(top, ss);
-    const RowScale k = row_scale<NORM>(value_of(top), ss, eps, H);
-    if (threadIdx.x == 0) scales[row] = k.scale;
+    const double a = value_of(top);
+    const float inv = inverse(a);
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
         const int i = (p * THREADS + threadIdx.x) * VEC;
         if (i >= H) continue;
         int n[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) n[e] = k.inv == 0.f ? 0 : quotient<NORM>(v[p][e], w[p][e], k.inv, k.a);
+        for (int e = 0; e < VEC; ++e) n[e] = inv == 0.f ? 0 : quotient<NORM>(v[p][e], w[p][e], inv, a);
         store_integers<VEC>(q + row * pitch + i, n);
     }
+    if (threadIdx.x == 0) scales[row] = row_scale<NORM>(a, ss, eps, H);
 }
 
 // The same for rows wider than a block's registers: read twice.
@@ -172,10 +172,11 @@ __global__ __launch_bounds__(1024) void wide_rows_q8_kernel(int8_t* __restrict__
         } else top = max(top, magnitude(v));
     }
     row_statistics<16, NORM>(top, ss);
-    const RowScale k = row_scale<NORM>(value_of(top), ss, eps, H);
-    if (threadIdx.x == 0) scales[row] = k.scale;
+    const double a = value_of(top);
+    const float inv = inverse(a);
     for (int i = threadIdx.x; i < H; i += 1024)                // (what a thread reads of the stream, it wrote itself)
-        q[row * pitch + i] = k.inv == 0.f ? (int8_t)0 : (int8_t)quotient<NORM>(to_f32<TX>(s[i]), NORM ? to_f32<TW>(weight[i]) : 1.f, k.inv, k.a);
+        q[row * pitch + i] = inv == 0.f ? (int8_t)0 : (int8_t)quotient<NORM>(to_f32<TX>(s[i]), NORM ? to_f32<TW>(weight[i]) : 1.f, inv, a);
+    if (threadIdx.x == 0) scales[row] = row_scale<NORM>(a, ss, eps, H);
 }
 
 template <typename TX, typename TD, typename TW, bool NORM>
