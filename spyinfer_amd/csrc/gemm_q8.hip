@@ -8,6 +8,12 @@
 // are 64 pieces of 16 bytes a load, which take the address unit 64 clocks: 64 rows, 12288 -> 4096 30.6 us for 20.7).  Piece p of row r of a tile
 // lies at place p ^ (r S / 4), so that the reads meet in no bank.  A wave keeps D units under way; units behind the end are loads beyond their buffers, which ask
 // the memory for nothing and bring zeros.
+//
+// What bounds it: few rows the matrix from memory (8 rows, 12288 -> 4096 9.6 us, 5.3 TB/s; 16 rows, gated, 4096 -> 2 x 12288 17.0 us, 5.9 TB/s) and a launch; 65 to
+// 500 rows the way of X and W from the L2s into the compute units: 200 rows, 4096 -> 6144 15.4 us, of which the matrix is 3.6 at the rate of a read and the
+// products 5; each of 192 blocks brings 0.8 MB, by 8 units of 24 KB a wave of which one is under way while one is multiplied.
+// Four waves a block: eight are slower, for all that they bring (16 rows, 12288 -> 4096 11.9 us for 11.6, 4096 -> 4096 6.4 for 6.1; 16 waves 11.8, 6.5);
+// so are units of one step of which two are under way (200 rows, 4096 -> 6144 19.6 for 17.2).
 #include "gemm_q8.h"
 
 // A tile of results: row tile i and column tile j of a block from (row0, 16 col0) on; lane 16 g + r has row r and columns 4 g ..
