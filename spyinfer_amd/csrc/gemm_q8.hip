@@ -43,12 +43,21 @@ __device__ __forceinline__ void q8_wait_loads() {
     asm volatile("" ::: "memory");
 }
 
+// Two products of a row tile with two column tiles whose sums are held in accumulation registers: where a block's LDS leaves a SIMD one wave, the compiler
+// keeps the sums there and moves every one of them to and fro (64 products, 192 moves).  It does not see matrix instructions here and leaves out the
+// wait states behind an ordinary instruction that writes their operands, hence the first line, and those before the sums are read (the end of the loop).
+__device__ __forceinline__ void q8_mfma2_held(q8_i32x4_t& a, q8_i32x4_t& b, q8_i32x4_t w0, q8_i32x4_t w1, q8_i32x4_t x) {
+    asm volatile("s_nop 1\n\tv_mfma_i32_16x16x64_i8 %0, %2, %4, %0\n\tv_mfma_i32_16x16x64_i8 %1, %3, %4, %1" : "+a"(a), "+a"(b) : "v"(w0), "v"(w1), "v"(x));
+}
+
 // ONCE: W is read by one block only, and passes the caches by (up to 64 rows, matrices from memory: 16 rows, 4096 -> 2 x 12288 19.8 / 18.4 us).
 template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename TC>
 __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int n_rows,
                                                 int blocks, const GateAct& act) {
     constexpr int PAIR = EPI == Q8_GATED ? 2 : 1, NO = NT / PAIR, PIECES = 4 * S, RPI = 16 / S;            // pieces of a row, rows that a load brings
     constexpr int ITEMS = MT * NO, MOST = MT * S / PAIR, PHASE = ITEMS < MOST ? ITEMS : MOST, OPS = MT * S + NT * S;
+    constexpr bool HELD = MT >= 6;
+    static_assert(!HELD || NT % 2 == 0, "held sums go in pairs");
     static_assert(D >= 2 && D <= 3 && (D - 1) * OPS <= 63, "a wait counts the loads issued after those that it waits for");
     // (arrays of their own: reads of one that the compiler cannot tell from another would wait for that one's loads)
     __shared__ __align__(1024) char stage0[WAVES * MT * S * 1024];
@@ -116,7 +125,10 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[j][i] = q8_mfma(w[d][s][j], x[i], acc[j][i]);
+                    for (int j = 0; j < NT; j += HELD ? 2 : 1) {
+                        if constexpr (HELD) q8_mfma2_held(acc[j][i], acc[j + 1][i], w[d][s][j], w[d][s][j + 1], x[i]);
+                        else acc[j][i] = q8_mfma(w[d][s][j], x[i], acc[j][i]);
+                    }
             }
             __builtin_amdgcn_sched_barrier(0);       // (the stage has been read: the products wait for the reads)
             load(d, u + (D + d) * WAVES);
@@ -124,6 +136,7 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
     }
     if (tid < MT * 16) row_scales[tid] = scale;
     else if (tid < (MT + NT) * 16) col_scales[tid - MT * 16] = scale;
+    if constexpr (HELD) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");          // (the sums may be read)
     // nothing is under way into the stages when the sums go there
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     q8_i32x4_t* const red = reinterpret_cast<q8_i32x4_t*>(stage0);          // [WAVES][PHASE][PAIR][64]
@@ -149,7 +162,7 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
 }
 
 template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename TC>
-__global__ __launch_bounds__(WAVES * 64) void gemm_q8_kernel(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N,
+__global__ __launch_bounds__(WAVES * 64, 2) void gemm_q8_kernel(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N,
                                                                     int tiles, int chunks, int n_rows, int blocks, GateAct act) {
     q8_staged_block<WAVES, MT, NT, S, D, ONCE, EPI, TC>(C, X, sx, W, sw, M, N, tiles, chunks, n_rows, blocks, act);
 }
