@@ -10,8 +10,10 @@
 // the memory for nothing and bring zeros.
 //
 // What bounds it: few rows the matrix from memory (8 rows, 12288 -> 4096 9.6 us, 5.3 TB/s; 16 rows, gated, 4096 -> 2 x 12288 17.0 us, 5.9 TB/s) and a launch; 65 to
-// 500 rows the way of X and W from the L2s into the compute units: 200 rows, 4096 -> 6144 15.4 us, of which the matrix is 3.6 at the rate of a read and the
-// products 5; each of 192 blocks brings 0.8 MB, by 8 units of 24 KB a wave of which one is under way while one is multiplied.
+// 500 rows the way of X and W from the L2s into the compute units: 200 rows, 4096 -> 6144 14.2 us, of which the matrix is 3.6 at the rate of a read and the
+// products 5; each of 192 blocks brings 0.8 MB, and a block's way in and out is 3.5.  Without any loads (but their issue) it is 2.7 shorter, without those of X 2.7
+// more: four waves' loads of a kilobyte take the address unit 64 clocks.  Loads one by one between the products need units of one step, whose pieces are half
+// lines: 18.9 us for 16.6 (matrices from memory).
 // Four waves a block: eight are slower, for all that they bring (16 rows, 12288 -> 4096 11.9 us for 11.6, 4096 -> 4096 6.4 for 6.1; 16 waves 11.8, 6.5);
 // so are units of one step of which two are under way (200 rows, 4096 -> 6144 19.6 for 17.2).
 #include "gemm_q8.h"
@@ -193,17 +195,17 @@ static int split_launch(const Q8Args& a) {
 }
 
 // Which blocks: those with the least estimated time, us, of c[0] + c[1] r k + c[2] r + c[3] b k + c[4] x, b the blocks over 256 compute units, r that rounded up,
-// k the chunks of K; x: chunks of K that row tiles bring over the units, x k (tall blocks: b).  Fitted to 4500 products of 1 to 8192 rows, 16 to 34816 columns and K of 512 to 17408,
-// plain and gated, each with the matrices from memory, in every kind of block (6 to 19 % rms, the short products' least exactly); what it takes is 1.1 % slower on average than the
-// fastest kind, 6.6 % at the 95th percentile.  NT 100 + MT, or, tall, the row tiles alone.
+// k the chunks of K; x: chunks of K that row tiles bring over the units, x k (tall blocks: b).  Fitted to 5000 products of 1 to 8192 rows, 16 to 24576 columns and K of 512 to 17408,
+// plain and gated, each with the matrices from memory, in every kind of block that might do (5 to 19 % rms, the short products' least exactly); what it takes is 1.2 % slower on
+// average than the fastest kind, 7.8 % at the 95th percentile.  NT 100 + MT, or, tall, the row tiles alone.
 struct Q8Cost { int plan; float c[5]; };
 static const Q8Cost q8_costs[] = {
-    {101, {2.69f, 0.0642f, 0.357f, 0.0601f, 0.f}}, {102, {2.63f, 0.0924f, 0.604f, 0.0807f, 0.000247f}}, {103, {2.52f, 0.134f, 0.935f, 0.052f, 0.0149f}},
-    {104, {1.6f, 0.164f, 2.1f, 0.0426f, 0.0122f}}, {201, {2.87f, 0.112f, 0.106f, 0.0753f, 0.f}}, {202, {2.98f, 0.126f, 0.213f, 0.136f, 0.f}},
-    {203, {2.91f, 0.176f, 0.566f, 0.127f, 0.f}}, {204, {2.77f, 0.208f, 0.97f, 0.103f, 0.f}}, {206, {1.95f, 0.254f, 2.51f, 0.f, 0.0292f}},
-    {404, {3.58f, 0.273f, 1.29f, 0.2f, 0.f}}, {406, {1.79f, 0.371f, 4.28f, 0.f, 0.0375f}}, {408, {2.46f, 0.459f, 5.05f, 0.f, 0.0294f}},
-    {8, {2.09f, 0.999f, 4.72f, 0.637f, 2.45f}}, {10, {1.8f, 1.23f, 5.85f, 0.548f, 3.4f}}, {12, {1.49f, 1.4f, 6.95f, 0.631f, 3.75f}},
-    {14, {0.754f, 1.58f, 8.58f, 0.723f, 4.18f}}, {16, {0.0796f, 1.83f, 9.34f, 0.735f, 5.32f}},
+    {101, {2.83f, 0.0584f, 0.286f, 0.0616f, 0.f}}, {102, {2.68f, 0.0817f, 0.538f, 0.f, 0.0367f}}, {103, {2.62f, 0.111f, 0.828f, 0.f, 0.0305f}},
+    {104, {1.56f, 0.144f, 2.13f, 0.f, 0.03f}}, {201, {2.84f, 0.107f, 0.135f, 0.0716f, 0.f}}, {202, {2.81f, 0.117f, 0.327f, 0.093f, 0.f}},
+    {203, {2.99f, 0.146f, 0.513f, 0.0491f, 0.0217f}}, {204, {2.81f, 0.192f, 0.913f, 0.0609f, 0.013f}}, {206, {1.7f, 0.267f, 2.57f, 0.f, 0.0256f}},
+    {404, {3.5f, 0.281f, 1.33f, 0.145f, 0.f}}, {406, {1.85f, 0.349f, 4.07f, 0.f, 0.0382f}}, {408, {2.15f, 0.429f, 5.07f, 0.f, 0.0296f}},
+    {8, {1.87f, 0.955f, 4.36f, 0.651f, 2.03f}}, {10, {1.81f, 1.15f, 5.47f, 0.638f, 2.44f}}, {12, {1.26f, 1.33f, 6.87f, 0.699f, 2.61f}},
+    {14, {1.08f, 1.51f, 8.17f, 0.801f, 2.8f}}, {16, {0.754f, 1.75f, 8.42f, 0.846f, 3.81f}},
 };
 
 static int q8_plan(int M, int tiles, int chunks, int gated) {

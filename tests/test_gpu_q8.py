@@ -399,3 +399,38 @@ def test_blocks_that_do_not_exist_are_turned_away(monkeypatch):
         monkeypatch.setattr(ops, "Q8_PLAN", plan)
         with pytest.raises(ops.KernelError, match="no blocks|row tiles"):
             ops.linear_q8(x, w)
+
+
+def test_rows_and_results_beyond_32_bits():
+    """More than 2^31 bytes of rows, and more than 2^31 results: the last rows and columns are those of the rows alone."""
+    from spyinfer_amd.kernels import ops
+    dev = require_gpu()
+    g = torch.Generator(device=dev).manual_seed(9)
+    T, K = 140_000, 17_408
+    q = torch.randint(-128, 128, (T, K), device=dev, generator=g, dtype=torch.int8)
+    x = ops.Q8Rows(q, torch.rand(T, device=dev, generator=g), K)
+    w = ops.Q8Weight.from_values(torch.randint(-128, 128, (24, K), device=dev, generator=g, dtype=torch.int8), torch.rand(24, device=dev, generator=g))
+    y = ops.linear_q8(x, w, torch.float32)
+    for at in (0, 123_361, 123_370, T - 70):
+        assert torch.equal(y[at:at + 70], ops.linear_q8(ops.Q8Rows(q[at:at + 70], x.scales[at:at + 70].clone(), K), w, torch.float32))
+    del x, q, y, w
+    T, N = 270_001, 8200
+    q = torch.randint(-128, 128, (T, 256), device=dev, generator=g, dtype=torch.int8)
+    x = ops.Q8Rows(q, torch.rand(T, device=dev, generator=g), 256)
+    w = ops.Q8Weight.from_values(torch.randint(-128, 128, (N, 256), device=dev, generator=g, dtype=torch.int8), torch.rand(N, device=dev, generator=g))
+    y = ops.linear_q8(x, w)
+    for at in (0, 261_890, T - 70):
+        assert torch.equal(y[at:at + 70], ops.linear_q8(ops.Q8Rows(q[at:at + 70], x.scales[at:at + 70].clone(), 256), w))
+    del y
+    T, K = 530_000, 4096
+    s = torch.empty((T, K), device=dev)
+    s[:100].normal_(generator=g)
+    s[100:-100] = 0
+    s[-100:].normal_(generator=g)
+    weight = torch.ones(K, device=dev)
+    last = ops.quantize_rows(s[-100:].clone())
+    rows = ops.quantize_rows(s)
+    assert torch.equal(rows.values[-100:], last.values) and torch.equal(rows.scales[-100:], last.scales) and not rows.values[100:-100].any()
+    last = ops.add_rms_norm_q8(s[-100:].clone(), s[-100:].clone(), weight, EPS)
+    rows = ops.add_rms_norm_q8(s, s.clone(), weight, EPS)
+    assert torch.equal(rows.values[-100:], last.values) and torch.equal(rows.scales[-100:], last.scales)
