@@ -10,32 +10,13 @@
 // the memory for nothing and bring zeros.
 //
 // What bounds it: few rows the matrix from memory (8 rows, 12288 -> 4096 9.6 us, 5.3 TB/s; 16 rows, gated, 4096 -> 2 x 12288 17.0 us, 5.9 TB/s) and a launch; 65 to
-// 500 rows the way of X and W from the L2s into the compute units: 200 rows, 4096 -> 6144 14.2 us, of which the matrix is 3.6 at the rate of a read and the
-// products 5; each of 192 blocks brings 0.8 MB, and a block's way in and out is 3.5.  Without any loads (but their issue) it is 2.7 shorter, without those of X 2.7
+// 500 rows the way of X and W from the L2s into the compute units: 200 rows, 4096 -> 6144 12.9 us, of which the matrix is 3.6 at the rate of a read and the
+// products 5; each of 192 blocks brings 0.8 MB, and a block's way in and out is 2.3.  Without any loads (but their issue) it is 2.7 shorter, without those of X 2.7
 // more: four waves' loads of a kilobyte take the address unit 64 clocks.  Loads one by one between the products need units of one step, whose pieces are half
 // lines: 18.9 us for 16.6 (matrices from memory).
 // Four waves a block: eight are slower, for all that they bring (16 rows, 12288 -> 4096 11.9 us for 11.6, 4096 -> 4096 6.4 for 6.1; 16 waves 11.8, 6.5);
 // so are units of one step of which two are under way (200 rows, 4096 -> 6144 19.6 for 17.2).
 #include "gemm_q8.h"
-
-// A tile of results: row tile i and column tile j of a block from (row0, 16 col0) on; lane 16 g + r has row r and columns 4 g ..
-template <int EPI, int NT, int NO, typename TC>
-__device__ __forceinline__ void q8_store_tile(TC* C, const q8_i32x4_t& sum, const q8_i32x4_t& up, int i, int j, int row0, int col0, int rows, int N, int r, int g,
-                                              const float* row_scales, const float* col_scales, const GateAct& act) {
-    const int n = (col0 + j) * 16 + 4 * g;
-    const float fx = row_scales[i * 16 + r];
-    float y[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = q8_value<EPI>(act, sum[e], up[e], fx, col_scales[j * 16 + 4 * g + e], col_scales[(NT - NO + j) * 16 + 4 * g + e]);
-    if (i * 16 + r >= rows) return;
-    TC* o = C + (size_t)(row0 + i * 16 + r) * N + n;
-    if (N % 4 == 0 && (uintptr_t)C % (4 * sizeof(TC)) == 0) { if (n < N) Vec4<TC>::store(o, y); }
-    else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (n + e < N) o[e] = from_f32<TC>(y[e]);
-    }
-}
 
 // waits until at most N loads are under way (and for nothing else)
 template <int N>
@@ -57,7 +38,7 @@ template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename 
 __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int n_rows,
                                                 int blocks, const GateAct& act) {
     constexpr int PAIR = EPI == Q8_GATED ? 2 : 1, NO = NT / PAIR, PIECES = 4 * S, RPI = 16 / S;            // pieces of a row, rows that a load brings
-    constexpr int ITEMS = MT * NO, MOST = MT * S / PAIR, PHASE = ITEMS < MOST ? ITEMS : MOST, OPS = MT * S + NT * S;
+    constexpr int ITEMS = MT * NO, MOST = MT * S / PAIR, OPS = MT * S + NT * S;
     constexpr bool HELD = MT >= 6;
     static_assert(!HELD || NT % 2 == 0, "held sums go in pairs");
     static_assert(D >= 2 && D <= 3 && (D - 1) * OPS <= 63, "a wait counts the loads issued after those that it waits for");
@@ -139,26 +120,62 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
     if (tid < MT * 16) row_scales[tid] = scale;
     else if (tid < (MT + NT) * 16) col_scales[tid - MT * 16] = scale;
     if constexpr (HELD) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");          // (the sums may be read)
-    // nothing is under way into the stages when the sums go there
+    // Nothing is under way into the stages when the sums go there, a wave's into the parts that it had to itself: tile t's at place t of the first, then of the
+    // second, sum (row r, columns 4 g ..) at place r ^ (its lane in a row of readers) of the sixteen of g.  A row's results of a tile row are L readers' of V
+    // neighbouring columns, so that a store is whole lines where the block has four column tiles (200 rows, 4096 -> 6144 15.5 us; tile by tile, 32 bytes of
+    // a row, in two rounds of one stage: 16.7).
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    q8_i32x4_t* const red = reinterpret_cast<q8_i32x4_t*>(stage0);          // [WAVES][PHASE][PAIR][64]
+    constexpr int V = NO == 1 ? 4 : 16 / (int)sizeof(TC), L = NO * 16 / V, TURN = 16 / L;
+    static_assert(L * TURN == 16 && ITEMS <= 2 * MOST, "readers of a row; tiles in two stages");
 #pragma unroll
-    for (int t0 = 0; t0 < ITEMS; t0 += PHASE) {
-        __syncthreads();
+    for (int t = 0; t < ITEMS; ++t)
 #pragma unroll
-        for (int t = t0; t < t0 + PHASE && t < ITEMS; ++t)
+        for (int p = 0; p < PAIR; ++p)
+            *reinterpret_cast<q8_i32x4_t*>(mine[t / MOST] + ((t % MOST * PAIR + p) * 64 + g * 16 + (r ^ (t % NO * 16 + 4 * g) / V * TURN)) * 16) = acc[p * NO + t % NO][t / NO];
+    __syncthreads();
+    // the sum of a row's places in the waves' parts, of column tile j from its column 4 q on
+    auto from = [&](int row, int j, int q) {
+        const int t = row / 16 * NO + j;
+        return (t < MOST ? stage0 + t * PAIR * 1024 : stage1 + (t - MOST) * PAIR * 1024) + (q * 16 + (row % 16 ^ (j * 16 + 4 * q) / V * TURN)) * 16;
+    };
+    auto add = [&](const char* at, auto kind) {
+        auto sum = *reinterpret_cast<const decltype(kind)*>(at);
 #pragma unroll
-            for (int p = 0; p < PAIR; ++p) red[((wave * PHASE + t - t0) * PAIR + p) * 64 + lane] = acc[p * NO + t % NO][t / NO];
-        __syncthreads();
-        for (int t = t0 + wave; t < min(t0 + PHASE, ITEMS); t += WAVES) {
-            q8_i32x4_t sum[PAIR];
+        for (int o = 1; o < WAVES; ++o) sum += *reinterpret_cast<const decltype(kind)*>(at + o * MT * S * 1024);
+        return sum;
+    };
+    const bool fours = N % 4 == 0 && (uintptr_t)C % (4 * sizeof(TC)) == 0, all = N % V == 0 && (uintptr_t)C % (V * sizeof(TC)) == 0;
+    if (fours) {
+        const int c = tid % L, n = col0 * 16 + c * V;
 #pragma unroll
-            for (int p = 0; p < PAIR; ++p) {
-                sum[p] = red[((t - t0) * PAIR + p) * 64 + lane];
+        for (int u = 0; u < MT * 16 * L; u += WAVES * 64) {
+            const int row = (u + tid) / L;
+            if (row >= rows) break;
+            const char* const at = from(row, c * V / 16, c * V % 16 / 4);
+            const float fx = row_scales[row];
+            float y[V];
 #pragma unroll
-                for (int u = 1; u < WAVES; ++u) sum[p] += red[((u * PHASE + t - t0) * PAIR + p) * 64 + lane];
+            for (int h = 0; h < V / 4; ++h) {
+                const q8_i32x4_t sum = add(at + h * 256, q8_i32x4_t{}), up = PAIR == 2 ? add(at + 1024 + h * 256, q8_i32x4_t{}) : sum;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[4 * h + e] = q8_value<EPI>(act, sum[e], up[e], fx, col_scales[c * V + 4 * h + e], col_scales[(NT - NO) * 16 + c * V + 4 * h + e]);
             }
-            q8_store_tile<EPI, NT, NO>(C, sum[0], sum[PAIR - 1], t / NO, t % NO, row0, col0, rows, N, r, g, row_scales, col_scales, act);
+            TC* const o = C + (size_t)(row0 + row) * N + n;
+            if (V * sizeof(TC) == 16 && all) {
+                if constexpr (V * sizeof(TC) == 16) if (n < N) q8_store_piece(o, y);
+            } else
+#pragma unroll
+                for (int h = 0; h < V; h += 4)
+                    if (n + h < N) Vec4<TC>::store(o + h, y + h);
+        }
+    } else {                                // a lane a column (200 rows, 2049 -> 4099 11.7 us; by readers of V columns, each stored by itself, 13.1)
+        const int c = tid % (NO * 16), n = col0 * 16 + c;
+        const float fw = col_scales[c], fu = col_scales[(NT - NO) * 16 + c];
+#pragma unroll 4
+        for (int row = tid / (NO * 16); row < rows; row += WAVES * 4 / NO) {
+            const char* const at = from(row, c / 16, c % 16 / 4) + c % 4 * 4;
+            const int sum = add(at, 0), up = PAIR == 2 ? add(at + 1024, 0) : sum;
+            if (n < N) C[(size_t)(row0 + row) * N + n] = from_f32<TC>(q8_value<EPI>(act, sum, up, row_scales[row], fw, fu));
         }
     }
 }
