@@ -4,6 +4,21 @@
 
 #define Q8_DIES 8
 
+// The block at place v of the order of which every die takes a run: bands of `high` rows of blocks, one column of blocks of a band behind the other.  The 32 or more
+// blocks that a die has at a time then read few rows of X and few columns of W.  (Whole columns, which read W into one L2 only, need many rows' X there at a time:
+// blocks of 128 x 64, 3503 rows, 9728 -> 1024 78 us for 52, 1400 rows, 4096 -> 4096 45 for 42; of 256 x 256, 8192 rows, 4096 -> 4096 121 for 112, 4096 rows, 12288 ->
+// 4096 152 for 148.  Bands of 8 and 16 of the former 51.5 and 57; of 4, 6 and 8 of 128 x 256, 4096 rows, 4096 -> 6144 100, 96.4 and 100, in one 120.)
+__device__ __forceinline__ void q8_block_at(int v, int n_rows, int n_cols, int high, int& row, int& col) {
+    int band = 0;
+    if (n_rows > high) {
+        band = v / (high * n_cols) * high;
+        v -= band * n_cols;
+        high = min(n_rows - band, high);
+    } else high = n_rows;
+    col = v / high;
+    row = band + v % high;
+}
+
 // One result: a sum times its row's and its column's scale; gated, the activation of the gate's times the up rows'.
 template <int EPI>
 __device__ __forceinline__ float q8_value(const GateAct& act, int a, int up, float fx, float fw, float fu) {

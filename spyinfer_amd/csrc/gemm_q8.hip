@@ -36,7 +36,7 @@ __device__ __forceinline__ void q8_mfma2_held(q8_i32x4_t& a, q8_i32x4_t& b, q8_i
 // ONCE: W is read by one block only, and passes the caches by (up to 64 rows, matrices from memory: 16 rows, 4096 -> 2 x 12288 19.8 / 18.4 us).
 template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename TC>
 __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int n_rows,
-                                                int blocks, const GateAct& act) {
+                                                int n_cols, const GateAct& act) {
     constexpr int PAIR = EPI == Q8_GATED ? 2 : 1, NO = NT / PAIR, PIECES = 4 * S, RPI = 16 / S;            // pieces of a row, rows that a load brings
     constexpr int ITEMS = MT * NO, MOST = MT * S / PAIR, OPS = MT * S + NT * S;
     constexpr bool HELD = MT >= 6;
@@ -47,11 +47,13 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
     __shared__ __align__(1024) char stage1[WAVES * MT * S * 1024];
     __shared__ __align__(1024) char stage2[D > 2 ? WAVES * MT * S * 1024 : 16];
     __shared__ float row_scales[MT * 16], col_scales[NT * 16];
-    const int per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;    // (a die takes a run of the blocks: gemm_q8_tall_kernel)
+    const int blocks = n_rows * n_cols, per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;    // (a die takes a run of the blocks)
     const int v = (blockIdx.x % Q8_DIES) * per + idx;
     if (idx >= per || v >= blocks) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4, tid = threadIdx.x;
-    const int col0 = v / n_rows * NO, row0 = (v % n_rows) * MT * 16, rows = min(M - row0, MT * 16);
+    int row_t, col_t;
+    q8_block_at(v, n_rows, n_cols, 4, row_t, col_t);
+    const int col0 = col_t * NO, row0 = row_t * MT * 16, rows = min(M - row0, MT * 16);
     static_assert(MT * 16 + NT * 16 <= WAVES * 64, "a thread for each scale");
     float scale = 0.f;
     if (tid < MT * 16) { if (tid < rows) scale = sx[row0 + tid]; }
@@ -182,8 +184,8 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
 
 template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename TC>
 __global__ __launch_bounds__(WAVES * 64, 2) void gemm_q8_kernel(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N,
-                                                                    int tiles, int chunks, int n_rows, int blocks, GateAct act) {
-    q8_staged_block<WAVES, MT, NT, S, D, ONCE, EPI, TC>(C, X, sx, W, sw, M, N, tiles, chunks, n_rows, blocks, act);
+                                                                    int tiles, int chunks, int n_rows, int n_cols, GateAct act) {
+    q8_staged_block<WAVES, MT, NT, S, D, ONCE, EPI, TC>(C, X, sx, W, sw, M, N, tiles, chunks, n_rows, n_cols, act);
 }
 
 struct Q8Args {
@@ -197,7 +199,7 @@ static int split_launch(const Q8Args& a) {
     const int64_t blocks = (int64_t)n_rows * n_cols;
     SPY_REQUIRE(blocks < (1 << 30), "spy_gemm_q8: %lld blocks", (long long)blocks);
     const unsigned grid = (unsigned)((blocks + Q8_DIES - 1) / Q8_DIES * Q8_DIES);
-#define SPLIT_ARGS(TC) (TC*)a.C, a.X, a.sx, a.W, a.sw, a.M, a.N, a.tiles, a.chunks, n_rows, (int)blocks, a.act
+#define SPLIT_ARGS(TC) (TC*)a.C, a.X, a.sx, a.W, a.sw, a.M, a.N, a.tiles, a.chunks, n_rows, n_cols, a.act
 #define SPLIT_BY(ONCE, EPI, TC) gemm_q8_kernel<4, MT, NT, S, D, ONCE, EPI, TC><<<grid, 256, 0, a.st>>>(SPLIT_ARGS(TC))
     // (more than four row tiles, or four column tiles, are for products of more rows)
 #define SPLIT(EPI, TC) do { if (n_rows == 1 && MT <= 4 && NT <= 2) SPLIT_BY((MT <= 4 && NT <= 2), EPI, TC); else SPLIT_BY(false, EPI, TC); } while (0)

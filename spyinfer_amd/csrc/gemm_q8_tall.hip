@@ -76,16 +76,18 @@ __device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t
 
 template <int MT, int EPI, typename TC>
 __global__ __launch_bounds__(256, 1) void gemm_q8_tall_kernel(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N,
-                                                              int tiles, int chunks, int n_rows, int n_cols, int blocks, GateAct act) {
+                                                              int tiles, int chunks, int n_rows, int n_cols, GateAct act) {
     __shared__ __align__(1024) bf16_t stage0[MT * 16 * 128];
     __shared__ __align__(1024) bf16_t stage1[MT * 16 * 128];
     __shared__ float row_scales[MT * 16];
-    // blocks go to the dies in turn: a die takes a run of the blocks in (columns, rows) order, so that a matrix' columns come into one L2 once
-    const int per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;
+    // blocks go to the dies in turn: a die takes a run of the blocks
+    const int blocks = n_rows * n_cols, per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;
     const int v = (blockIdx.x % Q8_DIES) * per + idx;
     if (idx >= per || v >= blocks) return;
-    const int col_t = v / n_rows, pitch = chunks * Q8_CHUNK;
-    const int row0 = min((v % n_rows) * MT * 16, M - MT * 16);          // the last rows' tile ends with row M - 1 (what it shares with the one before, both form alike)
+    const int pitch = chunks * Q8_CHUNK;
+    int row_t, col_t;
+    q8_block_at(v, n_rows, n_cols, 6, row_t, col_t);
+    const int row0 = min(row_t * MT * 16, M - MT * 16);          // the last rows' tile ends with row M - 1 (what it shares with the one before, both form alike)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (threadIdx.x < MT * 16) row_scales[threadIdx.x] = sx[row0 + threadIdx.x];              // (MT <= 16; behind the turns' barriers when it is read)
     const auto wres = __builtin_amdgcn_make_buffer_rsrc((void*)W, 0, tiles * chunks * 4096, 0x00020000);
@@ -115,7 +117,7 @@ static int tall_launch(void* C, int c_dtype, const int8_t* X, const float* sx, c
     const int64_t blocks = (int64_t)n_rows * n_cols;
     SPY_REQUIRE(M >= MT * 16 && blocks < (1 << 30), "spy_gemm_q8: %d rows in blocks of %d row tiles, %lld blocks", M, MT, (long long)blocks);
     const unsigned grid = (unsigned)((blocks + Q8_DIES - 1) / Q8_DIES * Q8_DIES);
-#define TALL(EPI, TC) gemm_q8_tall_kernel<MT, EPI, TC><<<grid, 256, 0, st>>>((TC*)C, X, sx, W, sw, M, N, tiles, chunks, n_rows, n_cols, (int)blocks, act)
+#define TALL(EPI, TC) gemm_q8_tall_kernel<MT, EPI, TC><<<grid, 256, 0, st>>>((TC*)C, X, sx, W, sw, M, N, tiles, chunks, n_rows, n_cols, act)
     if (gated) TALL(Q8_GATED, bf16_t);
     else if (c_dtype == SPY_F32) TALL(Q8_STORE, float);
     else TALL(Q8_STORE, bf16_t);

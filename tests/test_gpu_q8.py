@@ -363,9 +363,9 @@ PLANS = [101, 102, 103, 104, 201, 202, 203, 204, 206, 404, 406, 408, 8, 10, 12, 
 
 
 @pytest.mark.parametrize("plan", PLANS)
-@pytest.mark.parametrize("T,N,K", [(1, 40, 64), (16, 16, 1), (47, 100, 300), (64, 272, 2300), (130, 70, 1024), (259, 513, 777), (513, 33, 4200)])
+@pytest.mark.parametrize("T,N,K", [(1, 40, 64), (16, 16, 1), (47, 100, 300), (64, 272, 2300), (130, 70, 1024), (259, 513, 777), (513, 33, 4200), (2100, 550, 200)])
 def test_every_kind_of_block(plan, T, N, K, monkeypatch):
-    """Fewer rows, columns and chunks of K than a block has, and more of each; plain and gated, both result types."""
+    """Fewer rows, columns and chunks of K than a block has, and more of each, with more row blocks than a band; plain and gated, both result types."""
     from spyinfer_amd.kernels import ops
     dev = require_gpu()
     monkeypatch.setattr(ops, "Q8_PLAN", plan)
