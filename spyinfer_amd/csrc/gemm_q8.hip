@@ -6,13 +6,13 @@
 // waits for another before their sums are added, through LDS, at the end.  W goes from memory into operand registers, a kilobyte a load.  X goes through LDS, in a part that a
 // wave has to itself: its loads there bring whole pieces of 64 S bytes of a row, its reads from there are the operands (16 rows straight from memory
 // are 64 pieces of 16 bytes a load, which take the address unit 64 clocks: 64 rows, 12288 -> 4096 30.6 us for 20.7).  Piece p of row r of a tile
-// lies at place p ^ (r S / 4), so that the reads meet in no bank.  A wave keeps D units under way; units behind the end are loads beyond their buffers, which ask
+// lies at place p ^ (r S / 4), so that the reads meet in no bank.  A wave keeps two units under way; units behind the end are loads beyond their buffers, which ask
 // the memory for nothing and bring zeros.
 //
 // What bounds it: few rows the matrix from memory (8 rows, 12288 -> 4096 9.6 us, 5.3 TB/s; 16 rows, gated, 4096 -> 2 x 12288 17.0 us, 5.9 TB/s) and a launch; 65 to
-// 500 rows the way of X and W from the L2s into the compute units: 200 rows, 4096 -> 6144 12.9 us, of which the matrix is 3.6 at the rate of a read and the
-// products 5; each of 192 blocks brings 0.8 MB, and a block's way in and out is 2.3.  Without any loads (but their issue) it is 2.7 shorter, without those of X 2.7
-// more: four waves' loads of a kilobyte take the address unit 64 clocks.  Loads one by one between the products need units of one step, whose pieces are half
+// 500 rows the way of X and W from the L2s into the compute units: 200 rows, 4096 -> 6144 12.5 us, of which the matrix is 3.6 at the rate of a read and the
+// products 5; each of 256 blocks brings 0.7 MB, and a block's way in and out is 2.3.  (In blocks of 128 x 64, of which there are 192, 12.9; without any loads but their
+// issue those were 2.7 shorter, without those of X 2.7 more: four waves' loads of a kilobyte take the address unit 64 clocks.)  Loads one by one between the products need units of one step, whose pieces are half
 // lines: 18.9 us for 16.6 (matrices from memory).
 // Four waves a block: eight are slower, for all that they bring (16 rows, 12288 -> 4096 11.9 us for 11.6, 4096 -> 4096 6.4 for 6.1; 16 waves 11.8, 6.5);
 // so are units of one step of which two are under way (200 rows, 4096 -> 6144 19.6 for 17.2).
@@ -33,19 +33,21 @@ __device__ __forceinline__ void q8_mfma2_held(q8_i32x4_t& a, q8_i32x4_t& b, q8_i
     asm volatile("s_nop 1\n\tv_mfma_i32_16x16x64_i8 %0, %2, %4, %0\n\tv_mfma_i32_16x16x64_i8 %1, %3, %4, %1" : "+a"(a), "+a"(b) : "v"(w0), "v"(w1), "v"(x));
 }
 
+__device__ __forceinline__ void q8_mfma_held(q8_i32x4_t& a, q8_i32x4_t w, q8_i32x4_t x) {
+    asm volatile("s_nop 1\n\tv_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(a) : "v"(w), "v"(x));
+}
+
 // ONCE: W is read by one block only, and passes the caches by (up to 64 rows, matrices from memory: 16 rows, 4096 -> 2 x 12288 19.8 / 18.4 us).
-template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename TC>
+template <int WAVES, int MT, int NT, int S, bool ONCE, int EPI, typename TC>
 __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N, int tiles, int chunks, int n_rows,
                                                 int n_cols, const GateAct& act) {
     constexpr int PAIR = EPI == Q8_GATED ? 2 : 1, NO = NT / PAIR, PIECES = 4 * S, RPI = 16 / S;            // pieces of a row, rows that a load brings
-    constexpr int ITEMS = MT * NO, MOST = MT * S / PAIR, OPS = MT * S + NT * S;
+    constexpr int D = 2, ITEMS = MT * NO, MOST = MT * S / PAIR, OPS = MT * S + NT * S;
     constexpr bool HELD = MT >= 6;
-    static_assert(!HELD || NT % 2 == 0, "held sums go in pairs");
-    static_assert(D >= 2 && D <= 3 && (D - 1) * OPS <= 63, "a wait counts the loads issued after those that it waits for");
+    static_assert((D - 1) * OPS <= 63, "a wait counts the loads issued after those that it waits for");
     // (arrays of their own: reads of one that the compiler cannot tell from another would wait for that one's loads)
     __shared__ __align__(1024) char stage0[WAVES * MT * S * 1024];
     __shared__ __align__(1024) char stage1[WAVES * MT * S * 1024];
-    __shared__ __align__(1024) char stage2[D > 2 ? WAVES * MT * S * 1024 : 16];
     __shared__ float row_scales[MT * 16], col_scales[NT * 16];
     const int blocks = n_rows * n_cols, per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;    // (a die takes a run of the blocks)
     const int v = (blockIdx.x % Q8_DIES) * per + idx;
@@ -74,7 +76,7 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = q8_i32x4_t{0, 0, 0, 0};
-    char* const mine[3] = {stage0 + wave * MT * S * 1024, stage1 + wave * MT * S * 1024, stage2 + (D > 2 ? wave * MT * S * 1024 : 0)};
+    char* const mine[D] = {stage0 + wave * MT * S * 1024, stage1 + wave * MT * S * 1024};
     // A lane's own offset alone says whether a load lies in its buffer (the offset that all lanes share may not count): rows that do not exist, and whatever
     // belongs to a unit behind the end, lie beyond (2^30 is more than any block's rows, 2^31 more than any matrix)
     auto load = [&](int d, int unit) {
@@ -111,6 +113,7 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
                     for (int j = 0; j < NT; j += HELD ? 2 : 1) {
+                        if constexpr (HELD && NT % 2) { if (j + 1 == NT) { q8_mfma_held(acc[j][i], w[d][s][j], x[i]); break; } }
                         if constexpr (HELD) q8_mfma2_held(acc[j][i], acc[j + 1][i], w[d][s][j], w[d][s][j + 1], x[i]);
                         else acc[j][i] = q8_mfma(w[d][s][j], x[i], acc[j][i]);
                     }
@@ -128,7 +131,7 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
     // a row, in two rounds of one stage: 16.7).
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     constexpr int V = NO == 1 ? 4 : 16 / (int)sizeof(TC), L = NO * 16 / V, TURN = 16 / L;
-    static_assert(L * TURN == 16 && ITEMS <= 2 * MOST, "readers of a row; tiles in two stages");
+    static_assert(L * TURN <= 16 && ITEMS <= 2 * MOST, "readers of a row; tiles in two stages");
 #pragma unroll
     for (int t = 0; t < ITEMS; ++t)
 #pragma unroll
@@ -148,10 +151,9 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
     };
     const bool fours = N % 4 == 0 && (uintptr_t)C % (4 * sizeof(TC)) == 0, all = N % V == 0 && (uintptr_t)C % (V * sizeof(TC)) == 0;
     if (fours) {
-        const int c = tid % L, n = col0 * 16 + c * V;
 #pragma unroll
         for (int u = 0; u < MT * 16 * L; u += WAVES * 64) {
-            const int row = (u + tid) / L;
+            const int row = (u + tid) / L, c = (u + tid) % L, n = col0 * 16 + c * V;
             if (row >= rows) break;
             const char* const at = from(row, c * V / 16, c * V % 16 / 4);
             const float fx = row_scales[row];
@@ -171,28 +173,27 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
                     if (n + h < N) Vec4<TC>::store(o + h, y + h);
         }
     } else {                                // a lane a column (200 rows, 2049 -> 4099 11.7 us; by readers of V columns, each stored by itself, 13.1)
-        const int c = tid % (NO * 16), n = col0 * 16 + c;
-        const float fw = col_scales[c], fu = col_scales[(NT - NO) * 16 + c];
 #pragma unroll 4
-        for (int row = tid / (NO * 16); row < rows; row += WAVES * 4 / NO) {
+        for (int u = tid; u < rows * NO * 16; u += WAVES * 64) {
+            const int row = u / (NO * 16), c = u % (NO * 16), n = col0 * 16 + c;
             const char* const at = from(row, c / 16, c % 16 / 4) + c % 4 * 4;
             const int sum = add(at, 0), up = PAIR == 2 ? add(at + 1024, 0) : sum;
-            if (n < N) C[(size_t)(row0 + row) * N + n] = from_f32<TC>(q8_value<EPI>(act, sum, up, row_scales[row], fw, fu));
+            if (n < N) C[(size_t)(row0 + row) * N + n] = from_f32<TC>(q8_value<EPI>(act, sum, up, row_scales[row], col_scales[c], col_scales[(NT - NO) * 16 + c]));
         }
     }
 }
 
-template <int WAVES, int MT, int NT, int S, int D, bool ONCE, int EPI, typename TC>
+template <int WAVES, int MT, int NT, int S, bool ONCE, int EPI, typename TC>
 __global__ __launch_bounds__(WAVES * 64, 2) void gemm_q8_kernel(TC* C, const int8_t* X, const float* sx, const int8_t* W, const float* sw, int M, int N,
                                                                     int tiles, int chunks, int n_rows, int n_cols, GateAct act) {
-    q8_staged_block<WAVES, MT, NT, S, D, ONCE, EPI, TC>(C, X, sx, W, sw, M, N, tiles, chunks, n_rows, n_cols, act);
+    q8_staged_block<WAVES, MT, NT, S, ONCE, EPI, TC>(C, X, sx, W, sw, M, N, tiles, chunks, n_rows, n_cols, act);
 }
 
 struct Q8Args {
     void* C; int c_dtype; const int8_t* X; const float* sx; const int8_t* W; const float* sw; int M, N, tiles, chunks, gated; GateAct act; hipStream_t st;
 };
 
-template <int MT, int NT, int S, int D>
+template <int MT, int NT, int S>
 static int split_launch(const Q8Args& a) {
     const int no = a.gated ? NT / 2 : NT, col_tiles = a.gated ? a.tiles / 2 : a.tiles;
     const int n_rows = (a.M + MT * 16 - 1) / (MT * 16), n_cols = (col_tiles + no - 1) / no;
@@ -200,7 +201,7 @@ static int split_launch(const Q8Args& a) {
     SPY_REQUIRE(blocks < (1 << 30), "spy_gemm_q8: %lld blocks", (long long)blocks);
     const unsigned grid = (unsigned)((blocks + Q8_DIES - 1) / Q8_DIES * Q8_DIES);
 #define SPLIT_ARGS(TC) (TC*)a.C, a.X, a.sx, a.W, a.sw, a.M, a.N, a.tiles, a.chunks, n_rows, n_cols, a.act
-#define SPLIT_BY(ONCE, EPI, TC) gemm_q8_kernel<4, MT, NT, S, D, ONCE, EPI, TC><<<grid, 256, 0, a.st>>>(SPLIT_ARGS(TC))
+#define SPLIT_BY(ONCE, EPI, TC) gemm_q8_kernel<4, MT, NT, S, ONCE, EPI, TC><<<grid, 256, 0, a.st>>>(SPLIT_ARGS(TC))
     // (more than four row tiles, or four column tiles, are for products of more rows)
 #define SPLIT(EPI, TC) do { if (n_rows == 1 && MT <= 4 && NT <= 2) SPLIT_BY((MT <= 4 && NT <= 2), EPI, TC); else SPLIT_BY(false, EPI, TC); } while (0)
     if (a.gated) { if constexpr (NT % 2 == 0) SPLIT(Q8_GATED, bf16_t); else return spy_fail("spy_gemm_q8: a gated product by %d column tiles", NT); }
@@ -214,17 +215,18 @@ static int split_launch(const Q8Args& a) {
 }
 
 // Which blocks: those with the least estimated time, us, of c[0] + c[1] r k + c[2] r + c[3] b k + c[4] x, b the blocks over 256 compute units, r that rounded up,
-// k the chunks of K; x: chunks of K that row tiles bring over the units, x k (tall blocks: b).  Fitted to 5000 products of 1 to 8192 rows, 16 to 24576 columns and K of 512 to 17408,
-// plain and gated, each with the matrices from memory, in every kind of block that might do (5 to 19 % rms, the short products' least exactly); what it takes is 1.2 % slower on
-// average than the fastest kind, 7.8 % at the 95th percentile.  NT 100 + MT, or, tall, the row tiles alone.
+// k the chunks of K; x: chunks of K that row tiles bring over the units, x k (tall blocks: b).  Fitted to 6500 products of 1 to 8192 rows, 16 to 24576 columns and K of 512 to 17408,
+// plain and gated, with ten matrices in turn, in every kind of block that might do (6 to 16 % rms, the short products' least exactly); what it takes is 0.7 % slower on
+// average than the fastest kind, 5.3 % at the 95th percentile (without those of three column tiles and of five and seven row tiles 1.5 and 9 %; with blocks of one column
+// tile and two to four row tiles, of 2 x 6, 3 x 5 and 3 x 7 0.8 and 5.1 %).  NT 100 + MT, or, tall, the row tiles alone.
 struct Q8Cost { int plan; float c[5]; };
 static const Q8Cost q8_costs[] = {
-    {101, {2.83f, 0.0584f, 0.286f, 0.0616f, 0.f}}, {102, {2.68f, 0.0817f, 0.538f, 0.f, 0.0367f}}, {103, {2.62f, 0.111f, 0.828f, 0.f, 0.0305f}},
-    {104, {1.56f, 0.144f, 2.13f, 0.f, 0.03f}}, {201, {2.84f, 0.107f, 0.135f, 0.0716f, 0.f}}, {202, {2.81f, 0.117f, 0.327f, 0.093f, 0.f}},
-    {203, {2.99f, 0.146f, 0.513f, 0.0491f, 0.0217f}}, {204, {2.81f, 0.192f, 0.913f, 0.0609f, 0.013f}}, {206, {1.7f, 0.267f, 2.57f, 0.f, 0.0256f}},
-    {404, {3.5f, 0.281f, 1.33f, 0.145f, 0.f}}, {406, {1.85f, 0.349f, 4.07f, 0.f, 0.0382f}}, {408, {2.15f, 0.429f, 5.07f, 0.f, 0.0296f}},
-    {8, {1.87f, 0.955f, 4.36f, 0.651f, 2.03f}}, {10, {1.81f, 1.15f, 5.47f, 0.638f, 2.44f}}, {12, {1.26f, 1.33f, 6.87f, 0.699f, 2.61f}},
-    {14, {1.08f, 1.51f, 8.17f, 0.801f, 2.8f}}, {16, {0.754f, 1.75f, 8.42f, 0.846f, 3.81f}},
+    {101, {2.71f, 0.0579f, 0.409f, 0.0368f, 0.f}}, {201, {2.76f, 0.0945f, 0.277f, 0.0577f, 0.f}}, {202, {2.79f, 0.115f, 0.38f, 0.0784f, 0.f}},
+    {203, {2.84f, 0.148f, 0.543f, 0.0861f, 0.f}}, {204, {2.81f, 0.184f, 0.832f, 0.0907f, 0.f}}, {304, {3.34f, 0.221f, 0.966f, 0.113f, 0.f}},
+    {306, {2.03f, 0.3f, 3.13f, 0.0841f, 0.00869f}}, {308, {1.95f, 0.365f, 3.96f, 0.0647f, 0.0122f}}, {404, {3.43f, 0.282f, 1.13f, 0.108f, 0.f}},
+    {405, {1.76f, 0.337f, 3.45f, 0.133f, 0.f}}, {406, {1.7f, 0.342f, 3.72f, 0.164f, 0.f}}, {407, {1.7f, 0.387f, 4.29f, 0.133f, 0.00506f}},
+    {408, {1.73f, 0.412f, 4.7f, 0.162f, 0.00214f}}, {8, {1.62f, 1.02f, 4.09f, 0.554f, 2.91f}}, {10, {1.f, 1.19f, 5.84f, 0.606f, 2.88f}},
+    {12, {0.315f, 1.34f, 7.42f, 0.736f, 2.93f}}, {14, {0.0824f, 1.52f, 8.68f, 0.838f, 3.31f}}, {16, {0.f, 1.76f, 9.03f, 0.888f, 4.2f}},
 };
 
 static int q8_plan(int M, int tiles, int chunks, int gated) {
@@ -233,9 +235,9 @@ static int q8_plan(int M, int tiles, int chunks, int gated) {
     float least = INFINITY;
     for (const Q8Cost& p : q8_costs) {
         const bool tall = p.plan < 100;
-        const int MT = tall ? p.plan : p.plan % 100, NO = tall ? (gated ? 8 : 16) : p.plan / 100 / (gated ? 2 : 1);
-        // not many more row tiles than there are (four from 33 rows on, six from 81, eight from 113), tall blocks no more
-        if (NO < 1 || (tall ? M < 16 * MT : MT == 4 ? row_tiles < 3 : row_tiles < MT)) continue;
+        const int MT = tall ? p.plan : p.plan % 100, NT = tall ? 16 : p.plan / 100, NO = gated ? NT / 2 : NT;
+        // gate and up in pairs of column tiles; not many more row tiles than there are (four from 33 rows on, as many for more), tall blocks no more
+        if ((gated && NT % 2) || (tall ? M < 16 * MT : MT == 4 ? row_tiles < 3 : row_tiles < MT)) continue;
         const int cols = (col_tiles + NO - 1) / NO;
         const float blocks = (float)((row_tiles + MT - 1) / MT) * (float)cols / 256.f, rounds = ceilf(blocks), k = (float)chunks;
         const float us = p.c[0] + p.c[1] * rounds * k + p.c[2] * rounds + p.c[3] * blocks * k + p.c[4] * (tall ? blocks : (float)row_tiles * cols / 256.f * k);
@@ -259,18 +261,19 @@ extern "C" int spy_gemm_q8(void* C, int c_dtype, const void* X, const float* sx,
     if (!plan) plan = q8_plan(M, tiles, chunks, gated);
     if (plan >= 8 && plan <= 16) return q8_tall_launch(C, c_dtype, (const int8_t*)X, sx, (const int8_t*)W, sw, M, N, tiles, chunks, gated, act, plan, st);
     switch (plan) {
-        case 101: return split_launch<1, 1, 4, 2>(a);
-        case 102: return split_launch<2, 1, 2, 3>(a);
-        case 103: return split_launch<3, 1, 2, 3>(a);
-        case 104: return split_launch<4, 1, 2, 3>(a);
-        case 201: return split_launch<1, 2, 2, 2>(a);
-        case 202: return split_launch<2, 2, 2, 2>(a);
-        case 203: return split_launch<3, 2, 2, 2>(a);
-        case 204: return split_launch<4, 2, 2, 2>(a);
-        case 206: return split_launch<6, 2, 2, 2>(a);
-        case 404: return split_launch<4, 4, 2, 2>(a);
-        case 406: return split_launch<6, 4, 2, 2>(a);
-        case 408: return split_launch<8, 4, 2, 2>(a);
+        case 101: return split_launch<1, 1, 4>(a);
+        case 201: return split_launch<1, 2, 2>(a);
+        case 202: return split_launch<2, 2, 2>(a);
+        case 203: return split_launch<3, 2, 2>(a);
+        case 204: return split_launch<4, 2, 2>(a);
+        case 304: return split_launch<4, 3, 2>(a);
+        case 306: return split_launch<6, 3, 2>(a);
+        case 308: return split_launch<8, 3, 2>(a);
+        case 404: return split_launch<4, 4, 2>(a);
+        case 405: return split_launch<5, 4, 2>(a);
+        case 406: return split_launch<6, 4, 2>(a);
+        case 407: return split_launch<7, 4, 2>(a);
+        case 408: return split_launch<8, 4, 2>(a);
     }
     return spy_fail("spy_gemm_q8: no blocks by the name of %d", plan);
 }
