@@ -391,6 +391,24 @@ def test_every_kind_of_block(plan, T, N, K, monkeypatch):
     near(ops.linear_q8_gated(x, gated), activation64(want[:, :N], "silu") * want[:, N:], 2.0 ** -8 + 2.0 ** -13)
 
 
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("plan", PLANS)
+def test_results_that_begin_anywhere(plan, out, monkeypatch):
+    """A caller's tensor that begins at an odd place, at every second and at every fourth value; what lies around it stays."""
+    from spyinfer_amd.kernels import ops
+    dev = require_gpu()
+    monkeypatch.setattr(ops, "Q8_PLAN", plan)
+    T, N, K = 260, 200, 320
+    q, sx, p, sw = drawn(T, N, K, plan)
+    x, w = ops.Q8Rows.from_values(q.to(dev), sx.to(dev)), ops.Q8Weight.from_values(p.to(dev), sw.to(dev))
+    y = ops.linear_q8(x, w, out)
+    near(y, product64(q, sx, p, sw), (HALF[out] if out != torch.float32 else 0.0) + 3.1 * 2.0 ** -24)
+    for at in (1, 2, 4, 7):
+        held = torch.full((at + T * N + 9,), 7.0, dtype=out, device=dev)
+        ops.linear_q8(x, w, out, out=held[at:at + T * N].view(T, N))
+        assert torch.equal(held[at:at + T * N].view(T, N), y) and bool((held[:at] == 7).all()) and bool((held[at + T * N:] == 7).all())
+
+
 def test_blocks_that_do_not_exist_are_turned_away(monkeypatch):
     from spyinfer_amd.kernels import ops
     dev = require_gpu()
