@@ -14,7 +14,9 @@
 // products 5; each of 256 blocks brings 0.7 MB, and a block's way in and out is 2.3.  (In blocks of 128 x 64, of which there are 192, 12.9; without any loads but their
 // issue those were 2.7 shorter, without those of X 2.7 more: four waves' loads of a kilobyte take the address unit 64 clocks.)  Loads one by one between the products need units of one step, whose pieces are half
 // lines: 18.9 us for 16.6 (matrices from memory).
-// Four waves a block: eight are slower, for all that they bring (16 rows, 12288 -> 4096 11.9 us for 11.6, 4096 -> 4096 6.4 for 6.1; 16 waves 11.8, 6.5);
+// Blocks of one wave, which has all of K and adds nothing, for K up to 2048 (308 -> 4096, 735 rows 7.3 us; the best of four waves 10.8, tall 8.9): many lie on a compute unit,
+// and K is over before four waves have shared it.
+// Otherwise four waves a block: eight are slower, for all that they bring (16 rows, 12288 -> 4096 11.9 us for 11.6, 4096 -> 4096 6.4 for 6.1; 16 waves 11.8, 6.5);
 // so are units of one step of which two are under way (200 rows, 4096 -> 6144 19.6 for 17.2).
 #include "gemm_q8.h"
 
@@ -56,12 +58,17 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
     int row_t, col_t;
     q8_block_at(v, n_rows, n_cols, 4, row_t, col_t);
     const int col0 = col_t * NO, row0 = row_t * MT * 16, rows = min(M - row0, MT * 16);
-    static_assert(MT * 16 + NT * 16 <= WAVES * 64, "a thread for each scale");
-    float scale = 0.f;
-    if (tid < MT * 16) { if (tid < rows) scale = sx[row0 + tid]; }
-    else if (tid < (MT + NT) * 16) {
-        const int n = tid - MT * 16, tile = col0 + n / 16 % NO;
-        if (tile < tiles / PAIR) scale = sw[(n / 16 / NO * (tiles / PAIR) + tile) * 16 + n % 16];
+    constexpr int THREADS = WAVES * 64, SCALES = ((MT + NT) * 16 + THREADS - 1) / THREADS;
+    float scale[SCALES];
+#pragma unroll
+    for (int q = 0; q < SCALES; ++q) {
+        const int n = q * THREADS + tid - MT * 16;
+        scale[q] = 0.f;
+        if (n < 0) { if (n + MT * 16 < rows) scale[q] = sx[row0 + n + MT * 16]; }
+        else if (n < NT * 16) {
+            const int tile = col0 + n / 16 % NO;
+            if (tile < tiles / PAIR) scale[q] = sw[(n / 16 / NO * (tiles / PAIR) + tile) * 16 + n % 16];
+        }
     }
     const int w_bytes = tiles * chunks * 4096, pitch = chunks * Q8_CHUNK, n_units = chunks * 4 / S;
     const auto wres = __builtin_amdgcn_make_buffer_rsrc((void*)W, 0, w_bytes, 0x00020000);
@@ -122,8 +129,12 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
             load(d, u + (D + d) * WAVES);
         }
     }
-    if (tid < MT * 16) row_scales[tid] = scale;
-    else if (tid < (MT + NT) * 16) col_scales[tid - MT * 16] = scale;
+#pragma unroll
+    for (int q = 0; q < SCALES; ++q) {
+        const int n = q * THREADS + tid - MT * 16;
+        if (n < 0) row_scales[n + MT * 16] = scale[q];
+        else if (n < NT * 16) col_scales[n] = scale[q];
+    }
     if constexpr (HELD) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");          // (the sums may be read)
     // Nothing is under way into the stages when the sums go there, a wave's into the parts that it had to itself: tile t's at place t of the first, then of the
     // second, sum (row r, columns 4 g ..) at place r ^ (its lane in a row of readers) of the sixteen of g.  A row's results of a tile row are L readers' of V
@@ -193,7 +204,7 @@ struct Q8Args {
     void* C; int c_dtype; const int8_t* X; const float* sx; const int8_t* W; const float* sw; int M, N, tiles, chunks, gated; GateAct act; hipStream_t st;
 };
 
-template <int MT, int NT, int S>
+template <int MT, int NT, int S, int WAVES = 4>
 static int split_launch(const Q8Args& a) {
     const int no = a.gated ? NT / 2 : NT, col_tiles = a.gated ? a.tiles / 2 : a.tiles;
     const int n_rows = (a.M + MT * 16 - 1) / (MT * 16), n_cols = (col_tiles + no - 1) / no;
@@ -201,7 +212,7 @@ static int split_launch(const Q8Args& a) {
     SPY_REQUIRE(blocks < (1 << 30), "spy_gemm_q8: %lld blocks", (long long)blocks);
     const unsigned grid = (unsigned)((blocks + Q8_DIES - 1) / Q8_DIES * Q8_DIES);
 #define SPLIT_ARGS(TC) (TC*)a.C, a.X, a.sx, a.W, a.sw, a.M, a.N, a.tiles, a.chunks, n_rows, n_cols, a.act
-#define SPLIT_BY(ONCE, EPI, TC) gemm_q8_kernel<4, MT, NT, S, ONCE, EPI, TC><<<grid, 256, 0, a.st>>>(SPLIT_ARGS(TC))
+#define SPLIT_BY(ONCE, EPI, TC) gemm_q8_kernel<WAVES, MT, NT, S, ONCE, EPI, TC><<<grid, WAVES * 64, 0, a.st>>>(SPLIT_ARGS(TC))
     // (more than four row tiles, or four column tiles, are for products of more rows)
 #define SPLIT(EPI, TC) do { if (n_rows == 1 && MT <= 4 && NT <= 2) SPLIT_BY((MT <= 4 && NT <= 2), EPI, TC); else SPLIT_BY(false, EPI, TC); } while (0)
     if (a.gated) { if constexpr (NT % 2 == 0) SPLIT(Q8_GATED, bf16_t); else return spy_fail("spy_gemm_q8: a gated product by %d column tiles", NT); }
@@ -215,18 +226,20 @@ static int split_launch(const Q8Args& a) {
 }
 
 // Which blocks: those with the least estimated time, us, of c[0] + c[1] r k + c[2] r + c[3] b k + c[4] x, b the blocks over 256 compute units, r that rounded up,
-// k the chunks of K; x: chunks of K that row tiles bring over the units, x k (tall blocks: b).  Fitted to 6500 products of 1 to 8192 rows, 16 to 24576 columns and K of 512 to 17408,
-// plain and gated, with ten matrices in turn, in every kind of block that might do (6 to 16 % rms, the short products' least exactly); what it takes is 0.7 % slower on
-// average than the fastest kind, 5.3 % at the 95th percentile (without those of three column tiles and of five and seven row tiles 1.5 and 9 %; with blocks of one column
-// tile and two to four row tiles, of 2 x 6, 3 x 5 and 3 x 7 0.8 and 5.1 %).  NT 100 + MT, or, tall, the row tiles alone.
+// k the chunks of K; x: chunks of K that row tiles bring over the units, x k (tall blocks: b; blocks of one wave: k).  Fitted to 11000 products of 1 to 8192 rows, 16 to 24576
+// columns and K of 16 to 17408, plain and gated, with ten matrices in turn, in every kind of block that might do (6 to 12 % rms, the short products' least exactly); what it
+// takes is 0.7 % slower on average than the fastest kind, 5 % at the 95th percentile.  (Without blocks of three column tiles and of five and seven row tiles 1.5 and 9 %
+// from K = 512 on, with blocks of one column tile and two to four row tiles, of 2 x 6, 3 x 5 and 3 x 7 no better; without those of one wave 11 and 48 % up to there.)
+// NT 100 + MT, 1000 more for one wave, or, tall, the row tiles alone.
 struct Q8Cost { int plan; float c[5]; };
 static const Q8Cost q8_costs[] = {
-    {101, {2.71f, 0.0579f, 0.409f, 0.0368f, 0.f}}, {201, {2.76f, 0.0945f, 0.277f, 0.0577f, 0.f}}, {202, {2.79f, 0.115f, 0.38f, 0.0784f, 0.f}},
-    {203, {2.84f, 0.148f, 0.543f, 0.0861f, 0.f}}, {204, {2.81f, 0.184f, 0.832f, 0.0907f, 0.f}}, {304, {3.34f, 0.221f, 0.966f, 0.113f, 0.f}},
-    {306, {2.03f, 0.3f, 3.13f, 0.0841f, 0.00869f}}, {308, {1.95f, 0.365f, 3.96f, 0.0647f, 0.0122f}}, {404, {3.43f, 0.282f, 1.13f, 0.108f, 0.f}},
-    {405, {1.76f, 0.337f, 3.45f, 0.133f, 0.f}}, {406, {1.7f, 0.342f, 3.72f, 0.164f, 0.f}}, {407, {1.7f, 0.387f, 4.29f, 0.133f, 0.00506f}},
-    {408, {1.73f, 0.412f, 4.7f, 0.162f, 0.00214f}}, {8, {1.62f, 1.02f, 4.09f, 0.554f, 2.91f}}, {10, {1.f, 1.19f, 5.84f, 0.606f, 2.88f}},
-    {12, {0.315f, 1.34f, 7.42f, 0.736f, 2.93f}}, {14, {0.0824f, 1.52f, 8.68f, 0.838f, 3.31f}}, {16, {0.f, 1.76f, 9.03f, 0.888f, 4.2f}},
+    {101, {2.66f, 0.0578f, 0.466f, 0.0347f, 0.f}}, {201, {2.78f, 0.0919f, 0.34f, 0.0535f, 0.f}}, {202, {2.84f, 0.11f, 0.473f, 0.0746f, 0.f}},
+    {203, {2.88f, 0.139f, 0.668f, 0.0851f, 0.f}}, {204, {2.82f, 0.174f, 0.965f, 0.0928f, 0.f}}, {304, {3.26f, 0.212f, 1.14f, 0.115f, 0.f}},
+    {306, {1.89f, 0.293f, 3.39f, 0.0819f, 0.00863f}}, {308, {1.79f, 0.36f, 4.27f, 0.0591f, 0.0123f}}, {404, {3.35f, 0.276f, 1.32f, 0.105f, 0.f}},
+    {405, {1.69f, 0.33f, 3.68f, 0.132f, 0.f}}, {406, {1.67f, 0.332f, 3.94f, 0.165f, 0.f}}, {407, {1.68f, 0.38f, 4.49f, 0.129f, 0.00524f}},
+    {408, {1.68f, 0.403f, 4.96f, 0.155f, 0.0032f}}, {1202, {2.94f, 0.0504f, 0.158f, 0.0781f, 0.281f}}, {1404, {3.88f, 0.f, 0.513f, 0.264f, 0.6f}},
+    {8, {2.08f, 0.989f, 3.91f, 0.619f, 2.6f}}, {10, {1.92f, 1.17f, 5.07f, 0.667f, 2.73f}}, {12, {1.85f, 1.32f, 5.77f, 0.799f, 3.15f}},
+    {14, {1.66f, 1.5f, 7.08f, 0.914f, 3.26f}}, {16, {1.43f, 1.74f, 7.64f, 0.978f, 3.84f}},
 };
 
 static int q8_plan(int M, int tiles, int chunks, int gated) {
@@ -234,13 +247,14 @@ static int q8_plan(int M, int tiles, int chunks, int gated) {
     int best = 0;
     float least = INFINITY;
     for (const Q8Cost& p : q8_costs) {
-        const bool tall = p.plan < 100;
-        const int MT = tall ? p.plan : p.plan % 100, NT = tall ? 16 : p.plan / 100, NO = gated ? NT / 2 : NT;
-        // gate and up in pairs of column tiles; not many more row tiles than there are (four from 33 rows on, as many for more), tall blocks no more
-        if ((gated && NT % 2) || (tall ? M < 16 * MT : MT == 4 ? row_tiles < 3 : row_tiles < MT)) continue;
+        const bool tall = p.plan < 100, one = p.plan > 1000;
+        const int MT = tall ? p.plan : p.plan % 100, NT = tall ? 16 : p.plan / 100 % 10, NO = gated ? NT / 2 : NT;
+        // gate and up in pairs of column tiles; not many more row tiles than there are (four from 33 rows on, as many for more), tall blocks no more;
+        // blocks of one wave, which has to walk all of K, up to K = 2048 (what was measured)
+        if ((gated && NT % 2) || (one && chunks > 8) || (tall ? M < 16 * MT : MT == 4 ? row_tiles < 3 : row_tiles < MT)) continue;
         const int cols = (col_tiles + NO - 1) / NO;
         const float blocks = (float)((row_tiles + MT - 1) / MT) * (float)cols / 256.f, rounds = ceilf(blocks), k = (float)chunks;
-        const float us = p.c[0] + p.c[1] * rounds * k + p.c[2] * rounds + p.c[3] * blocks * k + p.c[4] * (tall ? blocks : (float)row_tiles * cols / 256.f * k);
+        const float us = p.c[0] + p.c[1] * rounds * k + p.c[2] * rounds + p.c[3] * blocks * k + p.c[4] * (tall ? blocks : one ? k : (float)row_tiles * cols / 256.f * k);
         if (us < least) { least = us; best = p.plan; }
     }
     return best;
@@ -274,6 +288,8 @@ extern "C" int spy_gemm_q8(void* C, int c_dtype, const void* X, const float* sx,
         case 406: return split_launch<6, 4, 2>(a);
         case 407: return split_launch<7, 4, 2>(a);
         case 408: return split_launch<8, 4, 2>(a);
+        case 1202: return split_launch<2, 2, 2, 1>(a);
+        case 1404: return split_launch<4, 4, 2, 1>(a);
     }
     return spy_fail("spy_gemm_q8: no blocks by the name of %d", plan);
 }

@@ -359,7 +359,7 @@ def test_a_result_tensor_of_another_kind_is_turned_away():
 
 
 #: kinds of blocks of a product (csrc/gemm_q8.hip), and row tiles of each
-PLANS = [101, 201, 202, 203, 204, 304, 306, 308, 404, 405, 406, 407, 408, 8, 10, 12, 14, 16]
+PLANS = [101, 201, 202, 203, 204, 304, 306, 308, 404, 405, 406, 407, 408, 1202, 1404, 8, 10, 12, 14, 16]
 
 
 @pytest.mark.parametrize("plan", PLANS)
