@@ -12,11 +12,13 @@
 // What bounds it: few rows the matrix from memory (8 rows, 12288 -> 4096 9.6 us, 5.3 TB/s; 16 rows, gated, 4096 -> 2 x 12288 17.0 us, 5.9 TB/s) and a launch; 65 to
 // 500 rows the way of X and W from the L2s into the compute units: 200 rows, 4096 -> 6144 12.5 us, of which the matrix is 3.6 at the rate of a read and the
 // products 5; each of 256 blocks brings 0.7 MB, and a block's way in and out is 2.3.  (In blocks of 128 x 64, of which there are 192, 12.9; without any loads but their
-// issue those were 2.7 shorter, without those of X 2.7 more: four waves' loads of a kilobyte take the address unit 64 clocks.)  Loads one by one between the products need units of one step, whose pieces are half
+// issue those were 2.7 shorter, without those of X 2.7 more: four waves' loads of a kilobyte take the address unit 64 clocks.)  Loads one by one between the products
+// need units of one step, whose pieces are half
 // lines: 18.9 us for 16.6 (matrices from memory).
 // Blocks of one wave, which has all of K and adds nothing, for K up to 2048 (308 -> 4096, 735 rows 7.3 us; the best of four waves 10.8, tall 8.9): many lie on a compute unit,
 // and K is over before four waves have shared it.
-// Otherwise four waves a block: eight are slower, for all that they bring (16 rows, 12288 -> 4096 11.9 us for 11.6, 4096 -> 4096 6.4 for 6.1; 16 waves 11.8, 6.5);
+// Otherwise four waves a block: eight are slower, for all that they bring (16 rows, 12288 -> 4096 11.9 us for 11.6, 4096 -> 4096 6.4 for 6.1; 16 waves 11.8, 6.5), also
+// where there are few blocks (16 rows, 12288 -> 256 8.9 for 8.5);
 // so are units of one step of which two are under way (200 rows, 4096 -> 6144 19.6 for 17.2).
 #include "gemm_q8.h"
 
