@@ -37,14 +37,10 @@ def resolve_dtype(name) -> torch.dtype:
 def bind_weights(model: DecoderModel, weights, device, weight_copies: str = "both", matrix_precision: str = "stored") -> None:
     """``model.bind`` with the engine's choice of the forms in which matrices are kept (EngineConfig.weight_copies,
     EngineConfig.matrix_precision)."""
-    before = ops.ROW_MAJOR_WEIGHTS, ops.MATRICES_Q8
-    ops.ROW_MAJOR_WEIGHTS, ops.MATRICES_Q8 = weight_copies != "tiled", matrix_precision == "int8"
-    kept = ops.matrices_kept_q8()
-    try:
+    with ops.matrices_bound(rows=weight_copies != "tiled", q8=matrix_precision == "int8") as kept_q8:
         model.bind(weights, device)
-    finally:
-        ops.ROW_MAJOR_WEIGHTS, ops.MATRICES_Q8 = before
-    if matrix_precision == "int8" and ops.matrices_kept_q8() == kept:
+        none = matrix_precision == "int8" and kept_q8() == 0
+    if none:
         raise ValueError("matrix_precision 'int8': the model has no matrix that can be held in 8 bits (those of PagedAttention and GatedMLP can)")
 
 

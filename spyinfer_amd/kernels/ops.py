@@ -354,9 +354,9 @@ def tile_weight(w: torch.Tensor) -> Optional[torch.Tensor]:
     return w.view(N // 16, 16, K // 128, 4, 4, 8).permute(2, 0, 3, 4, 1, 5).contiguous().view(N, K)
 
 
-#: False while a model's weights are bound: a bfloat16 matrix that has a tiled copy is kept in that form only
-#: (``weight_forms``), which halves the weights' device memory; a product of many rows then restores the rows into a
-#: scratch tensor first (``TiledOnly.rows``), which costs a sixth more time in a prompt portion of 2048 tokens.
+#: False: a bfloat16 matrix that has a tiled copy is kept in that form only (``weight_forms``), which halves the weights' device
+#: memory; a product of many rows then restores the rows into a scratch tensor first (``TiledOnly.rows``), which costs a sixth more
+#: time in a prompt portion of 2048 tokens.  Where a model is bound its own choice stands instead (``matrices_bound``).
 ROW_MAJOR_WEIGHTS = True
 #: most rows that a product takes straight from the tiled copy when the rows of the matrix are not kept
 TILED_ONLY_DIRECT_ROWS = 64
@@ -410,29 +410,48 @@ class TiledOnly:
         return untile_weight(t, self._buf[:t.numel()].view(t.shape))
 
 
-#: True while a model's weights are bound: the matrices of the parts that ask for it are kept in 8-bit integers only
-MATRICES_Q8 = False
-_q8_kept = 0                  # matrices kept so since the process began
+class _Binding(threading.local):
+    """How the model that this thread binds keeps its matrices."""
+    rows = None                # whether beside a tiled copy (None: ROW_MAJOR_WEIGHTS)
+    q8 = False                 # whether in 8-bit integers only, where the parts ask for it
+    q8_kept = 0                # matrices kept so
 
 
-def matrices_kept_q8() -> int:
-    """How many matrices ``weight_forms`` has brought to 8 bits in this process: what binding a model adds to it is the
-    model's share."""
-    return _q8_kept
+_binding = _Binding()
+
+
+@contextlib.contextmanager
+def matrices_bound(rows: bool = True, q8: bool = False):
+    """What runs inside (on this thread; other threads may bind models of their own) binds a model's weights: ``rows``, matrices with a tiled
+    copy keep their rows as well; ``q8``, the matrices of the parts that ask for it are kept in 8-bit integers only.  Gives a function that says how many
+    have been kept so."""
+    b = _binding
+    before = b.rows, b.q8, b.q8_kept
+    b.rows, b.q8, b.q8_kept = rows, q8, 0
+    try:
+        yield lambda: b.q8_kept
+    finally:
+        b.rows, b.q8, b.q8_kept = before
+
+
+def __getattr__(name):
+    if name == "MATRICES_Q8":          # whether the model that this thread binds keeps matrices in 8 bits
+        return _binding.q8
+    raise AttributeError("module %r has no attribute %r" % (__name__, name))
 
 
 def weight_forms(w: torch.Tensor, keep_rows: bool = False, q8: bool = False, gated: bool = False):
-    """(matrix, tiled copy or None) as a part keeps them for ``linear``: both forms, or, with ROW_MAJOR_WEIGHTS off and
-    a tiled copy at hand, the tiled copy alone (the first member is then a TiledOnly).  ``keep_rows``: the rows are
-    needed for something else than products (an embedding table) and stay.  ``q8``: with MATRICES_Q8 on the matrix is
+    """(matrix, tiled copy or None) as a part keeps them for ``linear``: both forms, or, where the model that is bound keeps no rows
+    (``matrices_bound``, ROW_MAJOR_WEIGHTS) and a tiled copy is at hand, the tiled copy alone (the first member is then a TiledOnly).  ``keep_rows``: the rows are
+    needed for something else than products (an embedding table) and stay.  ``q8``: in a model that keeps matrices in 8 bits this one is
     kept as a ``Q8Weight`` alone (``gated``: of [gate | up] rows), which ``linear``, ``linear_few``, ``linear_parts`` and
     ``linear_swiglu`` take in a matrix' place."""
-    global _q8_kept
-    if q8 and MATRICES_Q8:
-        _q8_kept += 1
+    if q8 and _binding.q8:
+        _binding.q8_kept += 1
         return quantize_weight(w, gated), None
     tiled = tile_weight(w)
-    if tiled is not None and not ROW_MAJOR_WEIGHTS and not keep_rows:
+    rows = ROW_MAJOR_WEIGHTS if _binding.rows is None else _binding.rows
+    if tiled is not None and not rows and not keep_rows:
         return TiledOnly(tiled), tiled
     return w, tiled
 
