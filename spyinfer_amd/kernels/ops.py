@@ -2820,7 +2820,7 @@ class Q8Weight:
 
     @staticmethod
     def from_values(values: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> "Q8Weight":
-        """``values`` int8 [N, K] with a finite scale for each row, float32 [N]."""
+        """``values`` int8 [N, K] with a finite scale for each row, float32 [N]; both are copied."""
         _check(values.dim() == 2 and values.dtype == torch.int8 and values.numel() > 0, "Q8Weight: int8 values [N, K] expected")
         _check(tuple(scales.shape) == (values.shape[0],) and scales.dtype == torch.float32 and scales.device == values.device,
                "Q8Weight: a float32 scale for each row expected")
@@ -2836,9 +2836,11 @@ class Q8Weight:
             full[:, :half, :K] = values.reshape(halves, half, K)
             kept[:, :half] = scales.view(halves, half)
             values, scales = full, kept
+        else:
+            scales = scales.clone(memory_format=torch.contiguous_format)
         words = values.contiguous().view(-1).view(torch.int64) if values.data_ptr() % 8 == 0 else values.clone().view(-1).view(torch.int64)
         tiles = words.view(halves * rows // 16, 16, width // 256, 4, 4, 2).permute(2, 0, 3, 4, 1, 5).contiguous().view(torch.int8)
-        return Q8Weight(tiles, scales.reshape(-1).contiguous(), (N, K), gated)
+        return Q8Weight(tiles, scales.view(-1), (N, K), gated)
 
     def to_rows(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The matrix that the integers stand for, [N, K], each value rounded once to ``dtype``."""

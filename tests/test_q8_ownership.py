@@ -1,0 +1,21 @@
+"""Matrices and rows in 8-bit integers made from a caller's tensors: they hold values of their own whatever the size, the place and the order of
+the tensors, without a GPU."""
+import pytest
+import torch
+
+from spyinfer_amd.kernels.ops import Q8Rows, Q8Weight
+
+
+def drawn(N, K, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8), torch.rand(N, generator=g) + 0.5
+
+
+@pytest.mark.parametrize("N,K,gated", [(16, 256, False), (32, 256, True), (48, 512, False), (15, 256, False), (32, 255, True), (34, 256, True)])
+def test_a_matrix_stays_when_the_tensors_it_came_from_change(N, K, gated):
+    p, s = drawn(N, K)
+    want = p.double() * s.double()[:, None]
+    w = Q8Weight.from_values(p, s, gated)
+    s.fill_(7.0)
+    p.zero_()
+    assert torch.equal(w.to_rows(torch.float64), want)
