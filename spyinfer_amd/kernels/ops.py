@@ -2772,14 +2772,12 @@ class Q8Rows:
 
     @staticmethod
     def from_values(values: torch.Tensor, scales: torch.Tensor) -> "Q8Rows":
-        """``values`` int8 [T, K] with a scale for each row, float32 [T]."""
+        """``values`` int8 [T, K] with a scale for each row, float32 [T]; both are copied (the constructor keeps the tensors that it is given)."""
         _check(values.dim() == 2 and values.dtype == torch.int8 and values.shape[1] > 0, "Q8Rows: int8 values [T, K] expected")
         T, K = values.shape
-        if K % 256 or not values.is_contiguous() or values.data_ptr() % 16:
-            kept = torch.zeros((T, (K + 255) & -256), dtype=torch.int8, device=values.device)
-            kept[:, :K] = values
-            values = kept
-        return Q8Rows(values, scales, K)
+        kept = values.new_zeros((T, (K + 255) & -256)) if K % 256 else values.new_empty((T, K))
+        kept[:, :K] = values
+        return Q8Rows(kept, scales.clone(), K)
 
     def to_rows(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values that the rows stand for, [T, K], each rounded once to ``dtype``."""

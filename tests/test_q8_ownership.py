@@ -19,3 +19,13 @@ def test_a_matrix_stays_when_the_tensors_it_came_from_change(N, K, gated):
     s.fill_(7.0)
     p.zero_()
     assert torch.equal(w.to_rows(torch.float64), want)
+
+
+@pytest.mark.parametrize("K", [256, 512, 255, 40])
+def test_rows_stay_when_the_tensors_they_came_from_change(K):
+    q, s = drawn(5, K, 1)
+    want = q.double() * s.double()[:, None]
+    x = Q8Rows.from_values(q, s)
+    s.fill_(7.0)
+    q.zero_()
+    assert torch.equal(x.to_rows(torch.float64), want) and x.shape == (5, K)
