@@ -2836,8 +2836,10 @@ class Q8Weight:
             values, scales = full, kept
         else:
             scales = scales.clone(memory_format=torch.contiguous_format)
-        words = values.contiguous().view(-1).view(torch.int64) if values.data_ptr() % 8 == 0 else values.clone().view(-1).view(torch.int64)
-        tiles = words.view(halves * rows // 16, 16, width // 256, 4, 4, 2).permute(2, 0, 3, 4, 1, 5).contiguous().view(torch.int8)
+        values = values.contiguous()
+        if values.data_ptr() % 8 or values.storage_offset() % 8:              # (eight integers at a time)
+            values = values.clone(memory_format=torch.contiguous_format)
+        tiles = values.view(-1).view(torch.int64).view(halves * rows // 16, 16, width // 256, 4, 4, 2).permute(2, 0, 3, 4, 1, 5).contiguous().view(torch.int8)
         return Q8Weight(tiles, scales.view(-1), (N, K), gated)
 
     def to_rows(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
