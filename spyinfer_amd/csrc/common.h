@@ -140,6 +140,17 @@ __device__ __forceinline__ float gated_value_short(const GateAct& a, float z, fl
     return __builtin_amdgcn_div_fixupf(fmaf(fmaf(-d4, q, z4), r, q), d, z) * up;
 }
 
+// For kernels that write matrix instructions out: behind this the sums may be read, the longest product has ended.  Every sum goes through a statement behind
+// the wait, so that whatever reads one depends on it (a wait alone orders no registers, and the compiler does not know that the sums come late).
+template <typename SUM, int A, int B>
+__device__ __forceinline__ void sums_settle(SUM (&acc)[A][B]) {
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < A; ++j)
+#pragma unroll
+        for (int i = 0; i < B; ++i) asm volatile("" : "+a"(acc[j][i]));
+}
+
 // Dispatch on a dtype code: binds `T` in `body`.
 #define SPY_DISPATCH(code, T, ...)                  \
     if ((code) == SPY_F32) { typedef float T; __VA_ARGS__; } \

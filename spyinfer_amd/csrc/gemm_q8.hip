@@ -137,7 +137,7 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
         if (n < 0) row_scales[n + MT * 16] = scale[q];
         else if (n < NT * 16) col_scales[n] = scale[q];
     }
-    if constexpr (HELD) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");          // (the sums may be read)
+    if constexpr (HELD) sums_settle(acc);
     // Nothing is under way into the stages when the sums go there, a wave's into the parts that it had to itself: tile t's at place t of the first, then of the
     // second, sum (row r, columns 4 g ..) at place r ^ (its lane in a row of readers) of the sixteen of g.  A row's results of a tile row are L readers' of V
     // neighbouring columns, so that a store is whole lines where the block has four column tiles (200 rows, 4096 -> 6144 15.5 us; tile by tile, 32 bytes of

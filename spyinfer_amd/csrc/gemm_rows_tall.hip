@@ -24,7 +24,7 @@
 
 // Two products of a row tile, X's 16 rows with two column tiles of W.  The compiler does not see matrix instructions here and leaves out the
 // wait states between them and ordinary instructions: an operand's register that one has written needs two (a turn begins with them, and
-// inside of it there are none: tests/test_rows_tall_listing.py looks), and what reads the sums waits for the last product (gr_sums_settle).
+// inside of it there are none: tests/test_rows_tall_listing.py looks), and what reads the sums waits for the last product (sums_settle).
 // Two before every pair cost 3 to 9 %.
 __device__ __forceinline__ void gr_mfma2(gr_f32x4_t& a, gr_f32x4_t& b, gr_bf16x8_t w0, gr_bf16x8_t w1, gr_bf16x8_t x) {
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %2, %4, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %3, %4, %1" : "+a"(a), "+a"(b) : "v"(w0), "v"(w1), "v"(x));

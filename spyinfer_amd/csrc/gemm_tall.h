@@ -3,9 +3,6 @@
 #pragma once
 #include "common.h"
 
-// the sums may be read: the longest product has ended
-__device__ __forceinline__ void gr_sums_settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
-
 // All turns of a block: n of them, of 256 bytes of K (128 bfloat16 or 256 8-bit integers).  OP: the operands' and the sums' registers, and two products of
 // a row tile with two column tiles, the sums in accumulation registers (csrc/gemm_rows_tall.hip says why and what that asks of the code around it).  wres, w_lane, w_at, w_turn: W's buffer, this lane's bytes in a load, each column tile's place and a
 // turn's bytes.  load_x(stage, i, c): asks for row tile i of turn c, straight into LDS (a wave 4 of its 16 rows).  Ends with nothing under way,
@@ -80,7 +77,7 @@ __device__ __forceinline__ void gr_tall_turns(typename OP::sums_t (&acc)[4][MT],
         turn();
     }
     if (c < n) products(0, stage0, stage1, n - 1, n - 1);
-    gr_sums_settle();
+    sums_settle(acc);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
