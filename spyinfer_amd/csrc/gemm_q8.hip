@@ -52,7 +52,8 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
     // (arrays of their own: reads of one that the compiler cannot tell from another would wait for that one's loads)
     __shared__ __align__(1024) char stage0[WAVES * MT * S * 1024];
     __shared__ __align__(1024) char stage1[WAVES * MT * S * 1024];
-    __shared__ float row_scales[MT * 16], col_scales[NT * 16];
+    __shared__ float2 row_scales[MT * 16];
+    __shared__ float col_scales[NT * 16];
     const int blocks = n_rows * n_cols, per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;    // (a die takes a run of the blocks)
     const int v = (blockIdx.x % Q8_DIES) * per + idx;
     if (idx >= per || v >= blocks) return;
@@ -134,7 +135,7 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
 #pragma unroll
     for (int q = 0; q < SCALES; ++q) {
         const int n = q * THREADS + tid - MT * 16;
-        if (n < 0) row_scales[n + MT * 16] = scale[q];
+        if (n < 0) row_scales[n + MT * 16] = q8_row_scale(scale[q]);
         else if (n < NT * 16) col_scales[n] = scale[q];
     }
     if constexpr (HELD) sums_settle(acc);
@@ -169,7 +170,7 @@ __device__ __forceinline__ void q8_staged_block(TC* C, const int8_t* X, const fl
             const int row = (u + tid) / L, c = (u + tid) % L, n = col0 * 16 + c * V;
             if (row >= rows) break;
             const char* const at = from(row, c * V / 16, c * V % 16 / 4);
-            const float fx = row_scales[row];
+            const float2 fx = row_scales[row];
             float y[V];
 #pragma unroll
             for (int h = 0; h < V / 4; ++h) {

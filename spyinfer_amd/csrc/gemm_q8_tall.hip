@@ -20,9 +20,9 @@ struct TallQ8 {
 
 // A block's results through its LDS stage, as many row tiles at a time as fit, in a part that a wave has to itself: the sums go there as they are, and a short loop reads
 // pieces of rows, forms the values and stores whole lines.  A piece of four columns lies at place p ^ (row % 16).
-// sx: the block's row scales in LDS; sw: the column scales, those of the up rows `half` on; at: this wave's first column; columns: those that exist.
+// sx: the block's row scales (q8_row_scale) in LDS; sw: the column scales, those of the up rows `half` on; at: this wave's first column; columns: those that exist.
 template <int MT, int EPI, typename TC>
-__device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t* stage, TC* out, int64_t ld, int columns, int at, const float* sx, const float* sw,
+__device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t* stage, TC* out, int64_t ld, int columns, int at, const float2* sx, const float* sw,
                                                 int half, const GateAct& act, int lane, int wave) {
     constexpr int CT = MT / 4, VEC = 16 / sizeof(TC), PIECES = (EPI == Q8_GATED ? 32 : 64) / VEC, ROWS = 64 / PIECES;
     int* mine = reinterpret_cast<int*>(stage) + wave * CT * 16 * 64;
@@ -46,7 +46,7 @@ __device__ __forceinline__ void q8_tall_results(q8_i32x4_t (&acc)[4][MT], bf16_t
 #pragma unroll 2
             for (int row = lane / PIECES; row < here; row += ROWS) {
                 const int* from = mine + row * 64;
-                const float fx = sx[i0 * 16 + row];
+                const float2 fx = sx[i0 * 16 + row];
                 float v[VEC];
 #pragma unroll
                 for (int k = 0; k < VEC / 4; ++k) {
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256, 1) void gemm_q8_tall_kernel(TC* C, const int8_
                                                               int tiles, int chunks, int n_rows, int n_cols, GateAct act) {
     __shared__ __align__(1024) bf16_t stage0[MT * 16 * 128];
     __shared__ __align__(1024) bf16_t stage1[MT * 16 * 128];
-    __shared__ float row_scales[MT * 16];
+    __shared__ float2 row_scales[MT * 16];
     // blocks go to the dies in turn: a die takes a run of the blocks
     const int blocks = n_rows * n_cols, per = (blocks + Q8_DIES - 1) / Q8_DIES, idx = blockIdx.x / Q8_DIES;
     const int v = (blockIdx.x % Q8_DIES) * per + idx;
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256, 1) void gemm_q8_tall_kernel(TC* C, const int8_
     q8_block_at(v, n_rows, n_cols, 6, row_t, col_t);
     const int row0 = min(row_t * MT * 16, M - MT * 16);          // the last rows' tile ends with row M - 1 (what it shares with the one before, both form alike)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (threadIdx.x < MT * 16) row_scales[threadIdx.x] = sx[row0 + threadIdx.x];              // (MT <= 16; behind the turns' barriers when it is read)
+    if (threadIdx.x < MT * 16) row_scales[threadIdx.x] = q8_row_scale(sx[row0 + threadIdx.x]);              // (MT <= 16; behind the turns' barriers when it is read)
     const auto wres = __builtin_amdgcn_make_buffer_rsrc((void*)W, 0, tiles * chunks * 4096, 0x00020000);
     const auto xres = __builtin_amdgcn_make_buffer_rsrc((void*)(X + (size_t)row0 * pitch), 0, MT * 16 * pitch, 0x00020000);
     int w_at[4];                                       // this wave's column tiles; one that does not exist reads the last (nothing is stored)
