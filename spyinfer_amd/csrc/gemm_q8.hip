@@ -212,7 +212,7 @@ static int split_launch(const Q8Args& a) {
     const int no = a.gated ? NT / 2 : NT, col_tiles = a.gated ? a.tiles / 2 : a.tiles;
     const int n_rows = (a.M + MT * 16 - 1) / (MT * 16), n_cols = (col_tiles + no - 1) / no;
     const int64_t blocks = (int64_t)n_rows * n_cols;
-    SPY_REQUIRE(blocks < (1 << 30), "spy_gemm_q8: %lld blocks", (long long)blocks);
+    SPY_REQUIRE((blocks + Q8_DIES) * WAVES * 64 < (1ll << 32), "spy_gemm_q8: %lld blocks are more than a launch holds", (long long)blocks);
     const unsigned grid = (unsigned)((blocks + Q8_DIES - 1) / Q8_DIES * Q8_DIES);
 #define SPLIT_ARGS(TC) (TC*)a.C, a.X, a.sx, a.W, a.sw, a.M, a.N, a.tiles, a.chunks, n_rows, n_cols, a.act
 #define SPLIT_BY(ONCE, EPI, TC) gemm_q8_kernel<WAVES, MT, NT, S, ONCE, EPI, TC><<<grid, WAVES * 64, 0, a.st>>>(SPLIT_ARGS(TC))

@@ -115,7 +115,7 @@ static int tall_launch(void* C, int c_dtype, const int8_t* X, const float* sx, c
                        GateAct act, hipStream_t st) {
     const int n_rows = (M + MT * 16 - 1) / (MT * 16), n_cols = gated ? (N + 127) / 128 : (N + 255) / 256;
     const int64_t blocks = (int64_t)n_rows * n_cols;
-    SPY_REQUIRE(M >= MT * 16 && blocks < (1 << 30), "spy_gemm_q8: %d rows in blocks of %d row tiles, %lld blocks", M, MT, (long long)blocks);
+    SPY_REQUIRE(M >= MT * 16 && (blocks + Q8_DIES) * 256 < (1ll << 32), "spy_gemm_q8: %d rows in blocks of %d row tiles, %lld blocks", M, MT, (long long)blocks);
     const unsigned grid = (unsigned)((blocks + Q8_DIES - 1) / Q8_DIES * Q8_DIES);
 #define TALL(EPI, TC) gemm_q8_tall_kernel<MT, EPI, TC><<<grid, 256, 0, st>>>((TC*)C, X, sx, W, sw, M, N, tiles, chunks, n_rows, n_cols, act)
     if (gated) TALL(Q8_GATED, bf16_t);

@@ -218,18 +218,27 @@ static void rows_launch(int8_t* q, float* scales, TX* x, int64_t ldx, const TD* 
 #undef ROWS
 }
 
+// rows in one launch: one of 2^32 threads or more is none
+#define ROWS_AT_ONCE (1 << 21)
+
 extern "C" int spy_add_rmsnorm_q8(void* q, float* scales, float* stream, const void* delta, int delta_dtype, const void* weight, int weight_dtype, float eps,
                                   int T, int H, int64_t pitch, hipStream_t st) {
     SPY_REQUIRE(T > 0 && H > 0 && pitch >= H && pitch % 16 == 0 && (uintptr_t)q % 16 == 0, "spy_add_rmsnorm_q8: bad sizes %d x %d", T, H);
-    SPY_DISPATCH(delta_dtype, TD, SPY_DISPATCH(weight_dtype, TW, rows_launch<float, TD, TW, true>(
-        (int8_t*)q, scales, stream, (int64_t)H, (const TD*)delta, (const TW*)weight, eps, T, H, pitch, st)));
+    for (int64_t t = 0; t < T; t += ROWS_AT_ONCE) {
+        const int n = (int)min((int64_t)ROWS_AT_ONCE, T - t);
+        SPY_DISPATCH(delta_dtype, TD, SPY_DISPATCH(weight_dtype, TW, rows_launch<float, TD, TW, true>(
+            (int8_t*)q + t * pitch, scales + t, stream + t * H, (int64_t)H, delta ? (const TD*)delta + t * H : nullptr, (const TW*)weight, eps, n, H, pitch, st)));
+    }
     SPY_CHECK_LAUNCH("spy_add_rmsnorm_q8");
     return 0;
 }
 
 extern "C" int spy_quantize_rows(void* q, float* scales, const void* x, int x_dtype, int64_t ldx, int T, int H, int64_t pitch, hipStream_t st) {
     SPY_REQUIRE(T > 0 && H > 0 && pitch >= H && pitch % 16 == 0 && (uintptr_t)q % 16 == 0 && ldx >= H, "spy_quantize_rows: bad sizes %d x %d", T, H);
-    SPY_DISPATCH(x_dtype, TX, rows_launch<TX, float, float, false>((int8_t*)q, scales, (TX*)x, ldx, nullptr, nullptr, 0.f, T, H, pitch, st));
+    for (int64_t t = 0; t < T; t += ROWS_AT_ONCE) {
+        const int n = (int)min((int64_t)ROWS_AT_ONCE, T - t);
+        SPY_DISPATCH(x_dtype, TX, rows_launch<TX, float, float, false>((int8_t*)q + t * pitch, scales + t, (TX*)x + t * ldx, ldx, nullptr, nullptr, 0.f, n, H, pitch, st));
+    }
     SPY_CHECK_LAUNCH("spy_quantize_rows");
     return 0;
 }
