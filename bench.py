@@ -270,7 +270,8 @@ def design_compare(args) -> int:
         "metric": "prefill and decode tok/s of %s beside Qwen3 at equal width, layers, heads and feed-forward size" % design_name,
         "value": first[design]["decode_b8"]["tokens_per_s"], "unit": "tokens/s", "n_gpus": 1, "steps": max(16, args.steps // 4), "warmup": 8,
         "ms_per_step": first[design]["decode_b8"]["ms_per_step"], "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
-        "dtype": "bf16" if args.dtype == "bfloat16" else "fp32", "data": "synthetic (random weights, uniform-random token ids)",
+        "dtype": {"bfloat16": "bf16" if args.matrix_precision == "stored" else "bf16, layers' matrices int8", "float32": "fp32"}[args.dtype],
+        "data": "synthetic (random weights, uniform-random token ids)",
         "config": {"model": "%s / Qwen3 layer shapes" % design_name, "layers": layers, "vocab": vocab, "prompt_len": args.prompt_len,
                    "prefill_tokens": args.prefill_tokens, "window": 1024, "graphs": not args.enforce_eager, "parallelism": "single GPU"},
         "widths": results}))
@@ -298,6 +299,7 @@ def main() -> int:
                     help="every request's keys in one number of parts instead of the host's cut by the step's lengths (for comparison)")
     ap.add_argument("--enforce-eager", action="store_true")
     ap.add_argument("--weight-copies", default="both", choices=["both", "tiled"], help="EngineConfig.weight_copies")
+    ap.add_argument("--matrix-precision", default="stored", choices=["stored", "int8"], help="EngineConfig.matrix_precision")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--shape", default="8b", choices=sorted(SHAPES), help="layer sizes of the model")
     ap.add_argument("--serve", type=int, default=0, metavar="N",
@@ -338,9 +340,10 @@ def main() -> int:
     model = arch.build(cfg)
     run_dtype = torch.bfloat16 if args.dtype == "bfloat16" else torch.float32
     weights = random_tensors_on_device(model.weight_specs(), args.seed, run_dtype, dev)
-    bind_weights(model, weights, dev, args.weight_copies)
+    bind_weights(model, weights, dev, args.weight_copies, args.matrix_precision)
     del weights
     torch.cuda.empty_cache()
+    held_bytes = torch.cuda.memory_allocated(dev)
 
     points = [int(x) for x in args.points.split(",") if x.strip()]
     uneven = [int(x) for x in args.uneven.split(",") if x.strip()]
@@ -351,7 +354,7 @@ def main() -> int:
     eng._init_with_model(model, dev, dtype=args.dtype, max_model_len=args.context, kvcache_block_size=page,
                          num_kvcache_blocks=max(pages_per_req * max_batch, -(-args.prefill_tokens // page)) + 8, max_num_seqs=max_batch,
                          max_num_batched_tokens=max(16384, args.prefill_tokens), enforce_eager=args.enforce_eager, seed=args.seed,
-                         weight_copies=args.weight_copies)
+                         weight_copies=args.weight_copies, matrix_precision=args.matrix_precision)
     g = torch.Generator().manual_seed(args.seed)
 
     def prompts(n, length):
@@ -360,8 +363,11 @@ def main() -> int:
     act_bytes = 2 if args.dtype == "bfloat16" else 4
     L, H, I, V = cfg.num_hidden_layers, cfg.hidden_size, cfg.intermediate_size, cfg.vocab_size
     nq, nkv, d = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
-    layer_params = H * (nq + 2 * nkv) * d + nq * d * H + 3 * H * I + 2 * H + 2 * d
-    weight_bytes = (L * layer_params + H + V * H) * act_bytes              # every weight a decode step uses, once
+    matrix_params = H * (nq + 2 * nkv) * d + nq * d * H + 3 * H * I
+    matrix_bytes = matrix_params * act_bytes
+    if args.matrix_precision == "int8":
+        matrix_bytes = matrix_params + 4 * ((nq + 2 * nkv) * d + 2 * H + 2 * I)          # (a float32 scale for each row of a matrix)
+    weight_bytes = L * (matrix_bytes + (2 * H + 2 * d) * act_bytes) + (H + V * H) * act_bytes              # every weight a decode step uses, once
     kv_bytes_per_token = sum(s.page_bytes(1, run_dtype) for s in model.cache_specs() if s is not None and s.paged)
 
     def decode_run(batch, steps, warmup, lengths=None):
@@ -482,12 +488,14 @@ def main() -> int:
         "metric": "decode tok/s at batch %d (%s, %d-token prompts)" % (args.batch, shape_name, args.prompt_len),
         "value": round(value, 1), "unit": "tokens/s", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup,
         "ms_per_step": round(ms, 4), "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
-        "dtype": "bf16" if args.dtype == "bfloat16" else "fp32", "data": "synthetic (random weights, uniform-random token ids)",
+        "dtype": {"bfloat16": "bf16" if args.matrix_precision == "stored" else "bf16, layers' matrices int8", "float32": "fp32"}[args.dtype],
+        "data": "synthetic (random weights, uniform-random token ids)",
         "config": {"model": shape_name, "layers": L, "layers_of_model": model_layers, "hidden": H, "q_heads": nq,
                    "kv_heads": nkv, "head_dim": d, "intermediate": I, "vocab": V, "global_batch": args.batch,
                    "seq_len": args.context, "prompt_len": args.prompt_len, "mean_context": round(ctx, 1), "page_size": page,
                    "graphs": not args.enforce_eager, "run_ahead": bool(eng.run_ahead), "parallelism": "single GPU",
-                   "uneven_prompts": bool(args.spread), "keys_cut_by_host": bool(ops.DECODE_PIECES)},
+                   "matrix_precision": args.matrix_precision,
+                   "weights_held_gb": round(held_bytes / 1e9, 2), "uneven_prompts": bool(args.spread), "keys_cut_by_host": bool(ops.DECODE_PIECES)},
         "prefill": {"value": round(T / pf, 1), "tokens": T, "ms": round(pf * 1e3, 3),
                     "frac": round(pf_flops / pf / PEAK_FLOPS[args.dtype], 4),
                     "library_tflops": None if lib_flops is None else round(lib_flops / 1e12, 1),
