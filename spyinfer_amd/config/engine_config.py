@@ -45,8 +45,8 @@ class EngineConfig:
     weight_copies: str = "both"
     #: "stored": matrices have the precision of the model folder.  "int8": those of the attention and of the gated
     #: feed-forwards are held as 8-bit integers with a scale for each output channel, and their products are integer
-    #: products with rows brought to 8 bits as they come, a scale for each token; half the memory and the bytes of a
-    #: decode step, at the precision of 8-bit weights and activations.  bfloat16 engines only; the embedding, the output
+    #: products with rows brought to 8 bits as they come, a scale for each token; half the memory and the bytes of these
+    #: matrices, at the precision of 8-bit weights and activations.  bfloat16 engines only; the embedding, the output
     #: head and all other matrices stay as they are.
     matrix_precision: str = "stored"
 

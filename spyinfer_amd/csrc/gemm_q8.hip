@@ -1,5 +1,5 @@
 // Products of 8-bit integer rows with 8-bit integer matrices (q8.h has both forms), sums in 32-bit integers, which hold them exactly
-// (K < 2^17):  y[m][n] = sum * row scale * column scale, rounded once; or the gated pair of such values.
+// (K < 2^17):  y[m][n] = sum * row scale * column scale in float32 (three roundings), then rounded to the result's type; or the gated pair of such values.
 //
 // Few rows and some: a block has MT row tiles and NT column tiles (gated: the gate's and the up values' of the same columns).  Its four waves take units
 // of S steps of 64 of K in turn, each all of the block's tiles, so that every byte is loaded by the one wave that multiplies it, and no wave
@@ -10,11 +10,13 @@
 // the memory for nothing and bring zeros.
 //
 // What bounds it: few rows the matrix from memory (8 rows, 12288 -> 4096 9.6 us, 5.3 TB/s; 16 rows, gated, 4096 -> 2 x 12288 17.0 us, 5.9 TB/s) and a launch; 65 to
-// 500 rows the way of X and W from the L2s into the compute units: 200 rows, 4096 -> 6144 12.5 us, of which the matrix is 3.6 at the rate of a read and the
+// 500 rows the way of X and W from the L2s into the compute units: 200 rows, 4096 -> 6144 12.3 us (14.3 with the matrix from memory), of which the matrix is 3.6 at the rate of a read and the
 // products 5; each of 256 blocks brings 0.7 MB, and a block's way in and out is 2.3.  (In blocks of 128 x 64, of which there are 192, 12.9; without any loads but their
 // issue those were 2.7 shorter, without those of X 2.7 more: four waves' loads of a kilobyte take the address unit 64 clocks.)  Loads one by one between the products
-// need units of one step, whose pieces are half
-// lines: 18.9 us for 16.6 (matrices from memory).
+// of units of one step, whose pieces are half lines: 18.9 us for 16.6 (matrices from memory); between those of a unit's second step, whose operands are all in registers
+// by then, not tried.
+// 17 to 64 rows, with few columns: the blocks, of which there are as many as columns for all of K (2560 columns 160 of one column tile), leave compute units idle: 64 rows, 9728 -> 2560
+// 13.3 us, the matrix 3.6.
 // Blocks of one wave, which has all of K and adds nothing, for K up to 2048 (308 -> 4096, 735 rows 7.3 us; the best of four waves 10.8, tall 8.9): many lie on a compute unit,
 // and K is over before four waves have shared it.
 // Otherwise four waves a block: eight are slower, for all that they bring (16 rows, 12288 -> 4096 11.9 us for 11.6, 4096 -> 4096 6.4 for 6.1; 16 waves 11.8, 6.5), also
@@ -231,7 +233,9 @@ static int split_launch(const Q8Args& a) {
 // Which blocks: those with the least estimated time, us, of c[0] + c[1] r k + c[2] r + c[3] b k + c[4] x, b the blocks over 256 compute units, r that rounded up,
 // k the chunks of K; x: chunks of K that row tiles bring over the units, x k (tall blocks: b; blocks of one wave: k).  Fitted to 11000 products of 1 to 8192 rows, 16 to 24576
 // columns and K of 16 to 17408, plain and gated, with ten matrices in turn, in every kind of block that might do (6 to 12 % rms, the short products' least exactly); what it
-// takes is 0.7 % slower on average than the fastest kind, 5 % at the 95th percentile.  (Without blocks of three column tiles and of five and seven row tiles 1.5 and 9 %
+// takes is 0.7 % slower on average than the fastest kind, 5 % at the 95th percentile.  Most of those matrices fit the last cache, and no term has the bytes: where a matrix comes from
+// memory the estimates are up to two fifths short (16 rows, gated, 4096 -> 2 x 12288 10.8 us, measured 17 to 18; 1 row, 17408 -> 17408 30, 57), and the
+// choice is up to 6 % slower than the fastest kind (that row in blocks 201, 101 54 us; 64 rows, gated, 4096 -> 2 x 12288 in 404 27.1, 204 26.1).  (Without blocks of three column tiles and of five and seven row tiles 1.5 and 9 %
 // from K = 512 on, with blocks of one column tile and two to four row tiles, of 2 x 6, 3 x 5 and 3 x 7 no better; without those of one wave 11 and 48 % up to there.)
 // NT 100 + MT, 1000 more for one wave, or, tall, the row tiles alone.
 struct Q8Cost { int plan; float c[5]; };

@@ -6,7 +6,11 @@
 // exact there, and the maximum is one of them.
 // A row of zeros: q 0, scale 0.  A row with a NaN or an infinity: q 0, scale NaN, so that all that is made of it is NaN.
 //
+// (The norm of zeros with eps 0 is no number, and its scale NaN.)
+//
 // Bound by memory: a block takes a row, reads it once, holds it in registers while the maximum (and the sum of squares) goes round, and writes it.
+// 8192 x 4096 with a bfloat16 addend 66 us, 5.4 TB/s; rows of 2047 x 12288 bfloat16 16.2 (20.9 from memory).  Rows that a width or a place keeps from pieces of eight are bound by their
+// narrow loads and stores: 2962 x 5667 bfloat16, a value a load and a byte a store, 30 us (10 at the rate of a copy), norms of 4096 x 1001 and 1000 17.7 and 12.6 (9).
 #include "q8.h"
 #include <type_traits>
 

@@ -2928,8 +2928,8 @@ def _gemm_q8(name: str, x: Q8Rows, w: Q8Weight, out_dtype: torch.dtype, out: Opt
 
 
 def linear_q8(x: Q8Rows, w: Q8Weight, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """y = x . w^T of rows and a matrix in 8-bit integers: the sums of products are 32-bit integers, exact; a sum times its row's and
-    its column's scale is rounded once, to ``out_dtype`` (bfloat16 or float32).  ``out``: the result is written there."""
+    """y = x . w^T of rows and a matrix in 8-bit integers: the sums of products are 32-bit integers, exact; a sum, its row's
+    scale and its column's are multiplied in float32 (three roundings: the sum's and the two products'), and the result is rounded to ``out_dtype`` (bfloat16 or float32).  ``out``: the result is written there."""
     if not (isinstance(x, Q8Rows) and isinstance(w, Q8Weight)):
         raise KernelError("linear_q8: Q8Rows and a Q8Weight expected")
     if w.gated:
@@ -2940,8 +2940,8 @@ def linear_q8(x: Q8Rows, w: Q8Weight, out_dtype: torch.dtype = torch.bfloat16, o
 
 
 def linear_q8_gated(x: Q8Rows, w: Q8Weight, activation: str = "silu") -> torch.Tensor:
-    """act(x . Wgate^T) * (x . Wup^T) -> bfloat16 [M, N / 2] for a matrix of [gate | up] rows, the two values formed as in
-    ``linear_q8`` and rounded once, after the activation.  ``activation``: one of GATED_ACTIVATIONS."""
+    """act(x . Wgate^T) * (x . Wup^T) -> bfloat16 [M, N / 2] for a matrix of [gate | up] rows, the two values formed in
+    float32 as in ``linear_q8``, and the result rounded to bfloat16 after the activation.  ``activation``: one of GATED_ACTIVATIONS."""
     if not (isinstance(x, Q8Rows) and isinstance(w, Q8Weight)):
         raise KernelError("linear_q8_gated: Q8Rows and a Q8Weight expected")
     if not w.gated:
