@@ -1,8 +1,8 @@
 // Products of many rows in 8-bit integers (q8.h) by blocks of 8 to 16 row tiles and 256 columns, one a compute unit (gemm_tall.h).
 //
 // A lane's 16 bytes are 16 integers where they are 8 bfloat16 there, and an instruction of the same 16 clocks multiplies twice as many; so the bfloat16
-// products' turns stand as they are, of 256 bytes of K.  Measured: 4096 rows, 12288 -> 4096 145 to 151 us (2.7 to 2.8 POP/s; the library's 8192 x 8192 x 8192 of
-// integers 2.03, the first kernel here, whose waves took X's operands straight from memory, 1452 us), gated, 4096 -> 2 x 12288 322 to 345 us (2.4 to 2.6).
+// products' turns stand as they are, of 256 bytes of K.  Measured: 4096 rows, 12288 -> 4096 145 to 156 us by box and clock (2.6 to 2.8 POP/s; the library's 8192 x 8192 x 8192 of
+// integers 2.03, the first kernel here, whose waves took X's operands straight from memory, 1452 us), gated, 4096 -> 2 x 12288 322 to 348 us (2.4 to 2.6).
 // What bounds it: by the counters the matrix units are busy for 68 % of all clocks and the clock is 1.97 GHz; with half of the compute units at work a turn takes
 // 2.2 us, with all of them 3: the power.  Gated, the activations of a block's results cost 2 to 3 us of the 57 that it takes.  Operands read
 // five or seven row tiles ahead in place of three change nothing.
